@@ -13,7 +13,9 @@
  *
  * and the three prefill helper kernels of the LLaMA glue
  * (models/tilemix_llama.py:718-869: squared-mean RMSNorm, token-major rotary,
- * SiLU * up).
+ * SiLU * up).  What follows a prefill has no counterpart there: a paged 4-bit
+ * cache of K and V, its page tables, and the attention that decodes and continues
+ * prompts over it (tilemix_kv4_*).
  *
  * Conventions (all entry points):
  *   - Plain C types only: device pointers, element strides, sizes.  No torch
@@ -37,7 +39,7 @@
 extern "C" {
 #endif
 
-#define TILEMIX_ABI_VERSION 4
+#define TILEMIX_ABI_VERSION 5
 
 enum tilemix_status {
     TILEMIX_OK = 0,
@@ -257,10 +259,134 @@ int tilemix_rotary_f16(const tilemix_rotary_params* p, void* stream);
  */
 int tilemix_silu_mul_f16(const void* gate, const void* up, void* out, int64_t n, void* stream);
 
+/*
+ * The paged 4-bit KV cache.  A pool holds `pages` pages of `page_size` token rows
+ * (a multiple of 16) for each of `heads` KV heads.  A row's head_dim values (at most
+ * 128) are split into groups of 32 channels; NG = ceil(head_dim / 32).  A group has a
+ * scale s and a minimum m in fp16 and a 4-bit code n a channel:
+ *   x' = min(max(x, -65408), 65408)     (so that no value below overflows fp16)
+ *   m  = fp16(min x'),  s = fp16((max x' - min x') / 15)            (fp32, IEEE division)
+ *   n  = min(max(rint((x' - m) / s), 0), 15)                        (n = 0 where s = 0)
+ *   value = fp16(n s + m), rounded once
+ * A group with a NaN gets m = NaN and reads back as NaN.  Arrays, contiguous, the
+ * code arrays 16-byte aligned:
+ *   codes  [pages, heads, page_size, 16 NG] bytes, channel 2j in the low half of byte j
+ *   params [pages, heads, page_size, NG, 2] fp16: s, m
+ * A row's slot is page * page_size + row of the page.  A block table names the pages of
+ * each sequence in order, block_table[b * stride_table + i], i < table_columns; an entry
+ * outside [0, pages) has no rows (they read as zeros and count as masked).
+ *
+ * `dtype` is the type of the K/V, query and output values: 0 fp16, 1 bf16.
+ *
+ * store: row t of k and v [tokens, heads, head_dim] goes to slots[t]; a slot outside
+ * [0, pages * page_size) is skipped.  Slots of a call must differ: of two rows with one
+ * slot a mixture may remain.
+ * load: row t of k and v becomes token t - cu_seqlens[b] of the sequence b that holds it
+ * (cu_seqlens[b] <= t < cu_seqlens[b + 1], non-decreasing); rows in no sequence, or past a
+ * sequence's table, become zeros.
+ */
+typedef struct tilemix_kv4_rows_params {
+    void* k_codes;                /* uint8 [pages, heads, page_size, 16 NG]        */
+    void* k_params;               /* fp16 [pages, heads, page_size, NG, 2]         */
+    void* v_codes;
+    void* v_params;
+    void* k;                      /* [tokens, heads, head_dim]; store: read, load: written */
+    void* v;
+    const int64_t* slots;         /* store: [tokens]                               */
+    const int32_t* block_table;   /* load: [batch, table_columns]                  */
+    const int32_t* cu_seqlens;    /* load: [batch + 1]                             */
+    int64_t stride_k_token, stride_k_head;
+    int64_t stride_v_token, stride_v_head;
+    int64_t stride_table;
+    int64_t tokens;
+    int32_t pages, page_size, heads, head_dim;
+    int32_t batch, table_columns; /* load                                          */
+    int32_t dtype;
+} tilemix_kv4_rows_params;
+
+int tilemix_kv4_store(const tilemix_kv4_rows_params* p, void* stream);
+int tilemix_kv4_load(const tilemix_kv4_rows_params* p, void* stream);
+
+/*
+ * Attention of packed queries over the cache.  Sequence b has the keys 0 .. seq_lens[b] - 1
+ * and the queries cu_seqlens_q[b] .. cu_seqlens_q[b + 1] - 1 (NULL: b * max_seqlen_q and on);
+ * its nq queries are its last tokens, so that with `causal` query i sees the keys
+ * j <= seq_lens[b] - nq + i, and all of them without.  Grouped heads: query head h reads KV head
+ * h / (heads_q / heads_k).  out = softmax(sm_scale q k^T) v over the cache's values;
+ * a query that sees no key gets zeros, rows of `out` behind the last query stay as they are.
+ * At most max_seqlen_q queries and max_seqlen_k keys of a sequence are read.
+ * `workspace`: tilemix_kv4_attn_workspace(p) bytes (0: may be NULL), 16-byte aligned, written
+ * and read by this call alone.
+ */
+typedef struct tilemix_kv4_attn_params {
+    const void* q;                /* [tokens_q, heads_q, head_dim]                 */
+    void* out;                    /* [tokens_q, heads_q, head_dim]                 */
+    const void* k_codes;          /* as in tilemix_kv4_rows_params                 */
+    const void* k_params;
+    const void* v_codes;
+    const void* v_params;
+    const int32_t* block_table;   /* [batch, table_columns]                        */
+    const int32_t* seq_lens;      /* [batch]                                       */
+    const int32_t* cu_seqlens_q;  /* [batch + 1] or NULL                           */
+    void* workspace;
+    int64_t workspace_bytes;
+    int64_t stride_q_token, stride_q_head;
+    int64_t stride_o_token, stride_o_head;
+    int64_t stride_table;
+    int64_t tokens_q;
+    float sm_scale;
+    int32_t pages, page_size, heads_q, heads_k, head_dim;
+    int32_t batch, table_columns;
+    int32_t max_seqlen_q, max_seqlen_k;
+    int32_t causal;
+    int32_t dtype;
+} tilemix_kv4_attn_params;
+
+int tilemix_kv4_attn(const tilemix_kv4_attn_params* p, void* stream);
+/* Bytes of workspace that the call takes; -1 for invalid parameters. */
+int64_t tilemix_kv4_attn_workspace(const tilemix_kv4_attn_params* p);
+
+/*
+ * Page tables.  free_pages[0 .. *free_count - 1] is a stack of free pages, seq_lens[b] the
+ * tokens that sequence b holds, block_table its pages.
+ *
+ * extend: sequence b gets lens[b] more tokens.  With cu[0] = 0, cu[b + 1] = cu[b] +
+ * max(lens[b], 0) and need_b = ceil((seq_lens[b] + lens[b]) / page_size) - ceil(seq_lens[b] /
+ * page_size), b is granted its tokens if lens[b] >= 0, cu[b + 1] <= tokens, its pages fit
+ * table_columns, and the needs of the sequences up to and with b for which all that holds do
+ * not exceed *free_count (or need_b is 0).  The g-th page taken (in order of b) is
+ * free_pages[*free_count - 1 - g].  Written: slots[cu[b] + i] and positions[cu[b] + i] =
+ * seq_lens[b] + i of a granted sequence, -1 and 0 for every other one of the `tokens`
+ * entries; cu_seqlens[b] = min(cu[b], tokens); granted[b]; and, in place, the new entries of
+ * block_table, seq_lens and free_count.
+ * truncate: sequence b keeps min(seq_lens[b], max(lens[b], 0)) tokens; pages behind them go back
+ * to the stack in the opposite order of extend (which it undoes), their entries become -1.
+ * `ticket`: one int32 that is 0 before the first call and belongs to this set of tables.
+ */
+typedef struct tilemix_kv4_tables_params {
+    int32_t* block_table;         /* [batch, table_columns]                        */
+    int32_t* seq_lens;            /* [batch]                                       */
+    int32_t* free_pages;          /* [free_capacity]                               */
+    int32_t* free_count;          /* [1]                                           */
+    int32_t* ticket;              /* [1]                                           */
+    const int32_t* lens;          /* [batch]                                       */
+    int64_t* slots;               /* extend: [tokens]                              */
+    int64_t* positions;           /* extend: [tokens]                              */
+    int32_t* cu_seqlens;          /* extend: [batch + 1]                           */
+    int32_t* granted;             /* extend: [batch]                               */
+    int64_t stride_table;
+    int64_t tokens;
+    int32_t batch;                /* at most 4096                                  */
+    int32_t table_columns, page_size, free_capacity;
+} tilemix_kv4_tables_params;
+
+int tilemix_kv4_extend(const tilemix_kv4_tables_params* p, void* stream);
+int tilemix_kv4_truncate(const tilemix_kv4_tables_params* p, void* stream);
+
 /* Library introspection. */
 int tilemix_abi_version(void);
 /* sizeof() of the parameter structs as compiled into the library:
- * 0 = quant, 1 = attn, 2 = rmsnorm, 3 = rotary. */
+ * 0 = quant, 1 = attn, 2 = rmsnorm, 3 = rotary, 4 = kv4_rows, 5 = kv4_attn, 6 = kv4_tables. */
 int64_t tilemix_params_size(int which);
 const char* tilemix_last_error(void);
 

@@ -1,0 +1,498 @@
+"""The paged 4-bit KV cache on the GPU against its 64-bit definition (oracle/paged_int4_oracle.py)."""
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+from _paged_int4 import TYPES, make_pool, make_table, rounded, tolerance
+from oracle import paged_int4_oracle as P
+from tilemix_amd.attention.hip.paged_int4 import (PagedInt4Cache, PageTables, load_int4, paged_int4_attention,
+                                                  store_int4)
+
+pytestmark = pytest.mark.gpu
+
+
+def dev(a, dtype=None):
+    t = torch.from_numpy(np.array(a, order="C"))
+    return (t if dtype is None else t.to(dtype)).cuda()
+
+
+def ints(values):
+    return torch.tensor(values, dtype=torch.int32, device="cuda")
+
+
+def to_cache(pool, dim):
+    return PagedInt4Cache(*(dev(a) for a in pool), dim)
+
+
+class Call:
+    """One attention call: inputs on both sides, the 64-bit result and its tolerance."""
+
+    def __init__(self, lens, new, heads, kv_heads, dim, page=16, dtype="fp16", causal=True, scale=None, seed=0,
+                 max_k=None, max_q=None):
+        self.table, pages = make_table(lens, page, seed)
+        self.pool = make_pool(pages, kv_heads, dim, page, seed)
+        self.lens, self.new, self.dim, self.dtype, self.causal = lens, new, dim, dtype, causal
+        self.cu = np.concatenate([[0], np.cumsum(new)]).astype(np.int64)
+        q = np.random.default_rng(seed + 7).standard_normal((int(self.cu[-1]), heads, dim))
+        q[..., 7 % dim] *= 8.0
+        self.q = rounded(q, dtype)
+        self.scale = dim ** -0.5 if scale is None else scale
+        self.given_scale = scale
+        self.max_q = max(new, default=0) if max_q is None else max_q
+        self.max_k = max(lens, default=0) if max_k is None else max_k
+
+    def want(self):
+        ref, mag, size = P.attention(self.q, *self.pool, self.dim, self.table, self.lens, self.cu, self.max_q,
+                                     self.max_k, self.causal, self.scale)
+        return ref, tolerance(ref, mag, size, self.dim, self.dtype)
+
+    def device_args(self):
+        return (dev(self.q, TYPES[self.dtype]), to_cache(self.pool, self.dim), dev(self.table), ints(self.lens),
+                dev(self.cu, torch.int32), self.max_q, self.max_k)
+
+    def run(self, **kw):
+        return paged_int4_attention(*self.device_args(), causal=self.causal, sm_scale=self.given_scale, **kw)
+
+    def check(self, got=None):
+        got = self.run() if got is None else got
+        ref, tol = self.want()
+        assert got.dtype == TYPES[self.dtype] and got.shape == ref.shape
+        diff = np.abs(got.double().cpu().numpy() - ref)
+        assert np.isfinite(diff).all() and (diff <= tol).all(), f"worst {np.max(diff / tol):.2f} of the tolerance"
+
+
+# ---- page tables -------------------------------------------------------------------
+
+
+def host_tables(tables):
+    return (tables.block_table.tolist(), tables.seq_lens.tolist(), tables.free_pages.tolist(),
+            int(tables.free_count))
+
+
+@pytest.mark.parametrize("batch,page,pages,steps", [(1, 16, 4, 12), (3, 16, 9, 30), (65, 64, 300, 8), (300, 32, 999, 6),
+                                                    (513, 16, 100, 5), (4096, 16, 3000, 3)])
+def test_tables_follow_the_definition(batch, page, pages, steps):
+    """Random extensions (too long, negative and empty ones among them; too few pages) and cuts."""
+    rng = np.random.default_rng(batch)
+    columns = 7
+    tables = PageTables.empty(pages, batch, columns, page)
+    table, lens, stack, count = host_tables(tables)
+    for step in range(steps):
+        new = [int(x) for x in rng.choice([0, 1, 1, 2, page - 1, page, page + 1, 3 * page, 8 * page, -1], batch)]
+        tokens = max(0, sum(max(n, 0) for n in new) - int(rng.integers(0, 3) == 0) * page)
+        slots, positions, cu, granted, count = P.extend(table, lens, stack, count, new, page, tokens)
+        plan = tables.extend(ints(new), tokens)
+        assert plan.slots.tolist() == slots and plan.positions.tolist() == positions
+        assert plan.cu_seqlens.tolist() == cu and plan.granted.tolist() == granted
+        assert plan.slots.dtype == plan.positions.dtype == torch.int64
+        assert host_tables(tables)[0] == table and host_tables(tables)[1] == lens
+        assert int(tables.free_count) == count and tables.free_pages.tolist()[:count] == stack[:count]
+        keep = [int(x) for x in rng.choice([0, -5, 1, page, 10 * page, 10 * page, 10 * page], batch)]
+        count = P.truncate(table, lens, stack, count, keep, page)
+        tables.truncate(ints(keep))
+        assert host_tables(tables)[:2] == (table, lens)
+        assert int(tables.free_count) == count and tables.free_pages.tolist()[:count] == stack[:count]
+    used = [p for row in table for p in row if p >= 0]
+    assert sorted(used + stack[:count]) == list(range(pages))
+
+
+def test_tables_cut_undoes_an_extension():
+    tables = PageTables.empty(500, 40, 20, 16)
+    rng = np.random.default_rng(0)
+    tables.extend(ints(rng.integers(0, 90, 40).tolist()), 4000)
+    before = [t.clone() for t in (tables.block_table, tables.seq_lens, tables.free_pages, tables.free_count)]
+    tables.extend(ints(rng.integers(0, 70, 40).tolist()), 4000)
+    tables.truncate(before[1])
+    for a, b in zip(before, (tables.block_table, tables.seq_lens, tables.free_pages, tables.free_count)):
+        assert torch.equal(a, b)
+
+
+def test_tables_of_no_sequence_and_no_token():
+    tables = PageTables.empty(4, 0, 3, 16)
+    plan = tables.extend(ints([]), 0)
+    assert plan.cu_seqlens.tolist() == [0] and plan.granted.numel() == plan.slots.numel() == 0
+    tables.truncate(ints([]))
+    tables = PageTables.empty(4, 2, 3, 16)
+    plan = tables.extend(ints([0, 0]), 0)
+    assert plan.cu_seqlens.tolist() == [0, 0, 0] and plan.granted.tolist() == [1, 1]
+    plan = tables.extend(ints([0, 3]), 9)  # entries that no sequence needs
+    assert plan.slots.tolist() == [0, 1, 2] + [-1] * 6 and plan.positions.tolist() == [0, 1, 2] + [0] * 6
+
+
+def test_tables_with_state_out_of_range():
+    """Lengths, counts and pages that no call leaves behind stay within the arrays."""
+    tables = PageTables.empty(4, 3, 2, 16)
+    tables.seq_lens.copy_(ints([-7, 10 ** 9, 5]))
+    tables.free_count.fill_(1000)
+    tables.free_pages.copy_(ints([3, -9, 2 ** 31 - 1, 0]))
+    plan = tables.extend(ints([20, 2 ** 31 - 1, 1]), 64)
+    assert plan.granted.tolist() == [1, 0, 0]  # the second request's end is past num_tokens, and so is the third's
+    assert tables.block_table[0].tolist() == [0, 2 ** 31 - 1] and tables.seq_lens.tolist() == [20, 32, 5]
+    tables.truncate(ints([-3, 0, 0]))
+    assert tables.seq_lens.tolist() == [0, 0, 0] and int(tables.free_count) == 4
+
+
+# ---- rows ---------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dim,heads,page,dtype", [(128, 8, 64, "fp16"), (128, 1, 16, "bf16"), (96, 2, 32, "fp16"),
+                                                  (80, 3, 16, "bf16"), (64, 2, 48, "fp16"), (33, 2, 16, "fp16"),
+                                                  (32, 1, 16, "bf16"), (7, 2, 16, "fp16"), (1, 1, 16, "fp16")])
+def test_store_and_load(dim, heads, page, dtype):
+    """Stored rows are the definition's codes and parameters, bit for bit, others stay, and load
+    returns the values they stand for."""
+    lens = [1, 0, page, page + 1, 3 * page - 1, 37]
+    table, pages = make_table(lens, page, dim)
+    pool = make_pool(pages, heads, dim, page, dim)
+    before = [a.copy() for a in pool]
+    cache = to_cache(pool, dim)
+    rng = np.random.default_rng(dim)
+    slots = [int(table[b, t // page]) * page + t % page for b, n in enumerate(lens) for t in range(n)]
+    skipped = [-1, pages * page, -2 ** 40, 2 ** 40]
+    order = rng.permutation(len(slots) + len(skipped))
+    where = np.array(slots + skipped, dtype=np.int64)[order]
+    x = {}
+    for name in "kv":
+        v = rng.standard_normal((len(where), heads, dim)) * rng.choice([1e-3, 1.0, 300.0], (len(where), heads, 1))
+        v[0] = 0.0
+        v[1] = 5.0
+        v[2, :, 0] = 6e4
+        v[3, :, -1] = -6e4
+        x[name] = rounded(v, dtype)
+    store_int4(dev(x["k"], TYPES[dtype]), dev(x["v"], TYPES[dtype]), cache, dev(where))
+    for name, at in (("k", 0), ("v", 2)):
+        codes, params = P.quantise(x[name])
+        for t, slot in enumerate(where):
+            if 0 <= slot < pages * page:
+                before[at][slot // page, :, slot % page] = codes[t]
+                before[at + 1][slot // page, :, slot % page] = params[t]
+    for a, b in zip(before, (cache.k_codes, cache.k_params, cache.v_codes, cache.v_params)):
+        assert np.array_equal(a.view(np.uint8), b.cpu().numpy().view(np.uint8))
+    cu = np.concatenate([[0], np.cumsum(lens)])
+    for out_type in TYPES:
+        k, v = load_int4(cache, dev(table), ints(cu.tolist()), int(cu[-1]) + 5, dtype=TYPES[out_type])
+        for got, at in ((k, 0), (v, 2)):
+            want = np.zeros((int(cu[-1]) + 5, heads, dim))
+            for b, n in enumerate(lens):
+                want[cu[b]:cu[b + 1]] = P.read_rows(before[at], before[at + 1], dim, table[b], n, pages,
+                                                    page)[0].transpose(1, 0, 2)
+            assert got.dtype == TYPES[out_type]
+            assert np.array_equal(got.double().cpu().numpy(), rounded(want, out_type))
+
+
+def test_store_of_strided_and_special_rows():
+    """Head-major and sliced K and V; infinities and finite values past the limit are clamped, a NaN
+    makes its group NaN and no other."""
+    dim, heads, page = 128, 2, 16
+    pool = make_pool(3, heads, dim, page)
+    rng = np.random.default_rng(3)
+    big = rng.standard_normal((heads, 9, 2 * dim + 3))
+    big[0, 0, 5], big[1, 2, 40], big[0, 3, 70], big[1, 4, 3] = np.inf, -np.inf, np.nan, 65504.0
+    t = torch.from_numpy(big).half().cuda()
+    for k in (t.transpose(0, 1)[..., :dim], t.transpose(0, 1)[..., 3:dim + 3], t.transpose(0, 1)[..., 0:2 * dim:2]):
+        cache = to_cache(pool, dim)
+        store_int4(k, k.contiguous(), cache, torch.arange(4, 13).cuda())
+        codes, params = P.quantise(k.double().cpu().numpy())
+        for c, p in ((cache.k_codes, cache.k_params), (cache.v_codes, cache.v_params)):
+            got_c = torch.cat([c[0, :, 4:16], c[1, :, :0]], 1)[:, :9].transpose(0, 1).cpu().numpy()
+            got_p = p[0, :, 4:13].transpose(0, 1).cpu().numpy()
+            assert np.array_equal(got_c, codes)
+            assert np.array_equal(np.isnan(got_p), np.isnan(params))
+            assert np.array_equal(np.nan_to_num(got_p), np.nan_to_num(params))
+            assert np.isfinite(P.dequantise(got_c, got_p, dim)[~np.isnan(params).any((-1, -2))]).all()
+
+
+def test_store_rounding_of_every_quotient():
+    """Rows of fp16 neighbours of the code borders: the codes are those of an exact division."""
+    rng = np.random.default_rng(5)
+    dim, page, tokens = 128, 16, 512
+    low = rng.uniform(-4, 0, (tokens, 1, 4, 1))
+    span = np.float16(rng.uniform(0.01, 8, (tokens, 1, 4, 1))).astype(np.float64)
+    step = (span / 15).astype(np.float16).astype(np.float64)
+    x = low + (rng.integers(0, 15, (tokens, 1, 4, 32)) + 0.5) * step
+    x[..., 0], x[..., 1] = low[..., 0], (low + span)[..., 0]
+    x = rounded(x.reshape(tokens, 1, dim), "fp16")
+    cache = PagedInt4Cache.empty(tokens // page, 1, dim, page)
+    t = dev(x, torch.float16)
+    store_int4(t, t, cache, torch.arange(tokens).cuda())
+    codes, params = P.quantise(x)
+    assert np.array_equal(cache.k_codes.reshape(tokens, 1, -1).cpu().numpy(), codes)
+    assert np.array_equal(cache.v_params.reshape(tokens, 1, 4, 2).cpu().numpy(), params)
+
+
+def test_load_of_pages_that_are_not_there():
+    """Table entries out of range and tokens past the table's columns read as zeros."""
+    dim, page = 64, 16
+    pool = make_pool(4, 2, dim, page)
+    table = np.array([[2, -1, 4, 1], [2 ** 31 - 1, 0, -2 ** 31, 3]], dtype=np.int32)
+    cu = [0, 70, 130]
+    k, v = load_int4(to_cache(pool, dim), dev(table), ints(cu), 130)
+    for got, at in ((k, 0), (v, 2)):
+        want = np.concatenate([P.read_rows(pool[at], pool[at + 1], dim, table[b], cu[b + 1] - cu[b], 4,
+                                           page)[0].transpose(1, 0, 2) for b in range(2)])
+        assert np.array_equal(got.double().cpu().numpy(), want)
+    assert not v[64:70].any()
+
+
+# ---- attention ----------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("lens", [[1], [2, 0, 1], [15, 16, 17], [63, 64, 65], [127, 129, 255, 256, 257, 300]])
+@pytest.mark.parametrize("dim,heads,kv_heads", [(128, 6, 2), (64, 7, 1)])
+def test_decode(lens, dim, heads, kv_heads):
+    Call(lens, [1] * len(lens), heads, kv_heads, dim).check()
+
+
+@pytest.mark.parametrize("dim", [1, 8, 16, 31, 32, 40, 64, 72, 80, 96, 100, 112, 128])
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+def test_head_dims(dim, dtype):
+    Call([100, 37], [1, 3], 4, 2, dim, dtype=dtype, seed=dim).check()
+
+
+@pytest.mark.parametrize("heads,kv_heads", [(1, 1), (4, 4), (14, 2), (28, 4), (16, 1), (17, 1), (40, 2), (33, 1),
+                                            (130, 1)])
+def test_grouped_heads(heads, kv_heads):
+    """Up to, at and past the 16 and 32 rows of a block with a single query."""
+    Call([70, 5], [1, 1], heads, kv_heads, 64, seed=heads).check()
+
+
+@pytest.mark.parametrize("page", [16, 32, 48, 64, 128, 208])
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+def test_page_sizes(page, dtype):
+    """Pages that end inside a tile, whole tiles and more than one; 48 and 208 divide none."""
+    Call([500, 63, 1, 209], [1, 2, 1, 5], 6, 2, 128, page=page, dtype=dtype, seed=page).check()
+
+
+@pytest.mark.parametrize("new", [[2, 2, 2], [5, 1, 16], [17, 30, 70], [0, 64, 1], [70, 0, 33], [90, 200, 1]])
+@pytest.mark.parametrize("causal", [True, False])
+def test_several_queries(new, causal):
+    """Drafts and chunks; more queries than keys leave the first rows without any."""
+    Call([90, 200, 33], new, 6, 2, 128, causal=causal, seed=sum(new)).check()
+
+
+@pytest.mark.parametrize("new", [[300], [129, 1]])
+@pytest.mark.parametrize("dim,heads,kv_heads,dtype", [(128, 3, 1, "fp16"), (64, 4, 2, "bf16"), (96, 2, 1, "fp16"),
+                                                      (40, 5, 1, "bf16")])
+def test_chunks(new, dim, heads, kv_heads, dtype):
+    Call([700, 140][:len(new)], new, heads, kv_heads, dim, page=64, dtype=dtype, seed=dim).check()
+
+
+@pytest.mark.parametrize("lens,new,heads,kv_heads,dim", [([5000], [1], 4, 2, 64), ([9000, 33, 2100], [1, 1, 1], 2, 1, 128),
+                                                         ([6001], [4], 6, 1, 96), ([4097, 700], [40, 3], 2, 1, 32)])
+def test_long_sequences_are_split(lens, new, heads, kv_heads, dim):
+    Call(lens, new, heads, kv_heads, dim, page=64, seed=dim).check()
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.2, 0.5, 1e-30])
+def test_scales(scale):
+    Call([130, 20], [1, 4], 4, 2, 64, scale=scale, seed=11).check()
+
+
+def test_bounds_on_queries_and_keys():
+    """max_seqlen_q and max_seqlen_k cut; without cu_seqlens_q every sequence has max_seqlen_q queries."""
+    Call([300, 50], [1, 1], 4, 2, 64, max_k=130).check()
+    c = Call([100, 90], [3, 3], 4, 2, 64)
+    q, cache, table, lens, _, max_q, max_k = c.device_args()
+    c.check(paged_int4_attention(q, cache, table, lens, None, max_q, max_k))
+    c = Call([100, 90], [9, 3], 4, 2, 64, max_q=5)
+    args = c.device_args()
+    out = torch.full_like(args[0], 7.0)
+    got = paged_int4_attention(*args, out=out)
+    assert (got[5:9] == 7.0).all()
+    ref, tol = c.want()
+    diff = np.abs(got.double().cpu().numpy() - ref)
+    keep = [i for i in range(12) if not 5 <= i < 9]
+    assert (diff[keep] <= tol[keep]).all()
+
+
+def test_empty_calls():
+    c = Call([0, 0], [1, 2], 4, 2, 64)
+    assert not c.run().any()
+    pool = make_pool(2, 2, 64, 16)
+    q = torch.zeros(0, 4, 64, dtype=torch.float16, device="cuda")
+    none = torch.empty(0, 3, dtype=torch.int32, device="cuda")
+    assert paged_int4_attention(q, to_cache(pool, 64), none, ints([]), ints([0]), 1, 5).shape == q.shape
+    # a table without columns: no key
+    q = torch.ones(2, 4, 64, dtype=torch.float16, device="cuda")
+    none = torch.empty(2, 0, dtype=torch.int32, device="cuda")
+    assert not paged_int4_attention(q, to_cache(pool, 64), none, ints([5, 1]), None, 1, 5).any()
+
+
+def test_out_strides_and_rows_behind():
+    """q and out as slices of wider tensors, head-major, unaligned; rows behind the last query stay."""
+    c = Call([90, 40], [2, 1], 4, 2, 64, seed=2)
+    q, *rest = c.device_args()
+    wide = torch.zeros(5, 4, 200, dtype=torch.float16, device="cuda")
+    for at in (0, 3, 8):
+        wide[:3, :, at:at + 64] = q
+        out = torch.full((4, 5, 77), 9.0, dtype=torch.float16, device="cuda").transpose(0, 1)
+        got = paged_int4_attention(wide[:, :, at:at + 64], *rest, out=out[:, :, 5:69])
+        assert got.data_ptr() == out[:, :, 5:69].data_ptr()
+        c.check(got[:3])
+        assert (out[3:] == 9.0).all() and (out[:, :, :5] == 9.0).all() and (out[:, :, 69:] == 9.0).all()
+    split = q.repeat(1, 1, 2)[:, :, ::2]  # no unit stride: copied
+    assert split.stride(2) == 2
+    assert torch.equal(paged_int4_attention(split, *rest), paged_int4_attention(split.contiguous(), *rest))
+
+
+def test_bad_pages_are_not_seen():
+    """Table entries out of range, in the middle and for a whole sequence."""
+    c = Call([200, 100, 60], [1, 2, 1], 4, 2, 64, seed=4)
+    c.table[0, 1], c.table[0, 5], c.table[0, 12] = -1, 10 ** 9, -2 ** 31
+    c.table[2, :] = 2 ** 31 - 1
+    c.check()
+    assert not c.run()[3].any()
+
+
+@pytest.mark.parametrize("where", ["params", "both"])
+def test_what_lies_behind_the_end_is_not_seen(where):
+    """Rows behind a sequence's last token hold NaN scales and any codes."""
+    c = Call([70, 16, 33], [3, 1, 20], 4, 2, 128, seed=5)
+    good = c.run()
+    page = 16
+    bad = [a.copy() for a in c.pool]
+    used = set()
+    for b, n in enumerate(c.lens):
+        for t in range(n):
+            used.add((int(c.table[b, t // page]), t % page))
+    for p in range(bad[0].shape[0]):
+        for r in range(page):
+            if (p, r) not in used:
+                for i in (1, 3):
+                    bad[i][p, :, r] = np.nan
+                if where == "both":
+                    bad[0][p, :, r] = bad[2][p, :, r] = 255
+    c.pool = bad
+    assert torch.equal(c.run(), good)
+
+
+def test_nan_reaches_the_queries_that_see_it():
+    """A NaN in K: all of a query's channels.  In V: the group's channels.  Earlier queries: none."""
+    for at, kind in ((195, "k"), (195, "v"), (20, "v"), (199, "v")):
+        c = Call([200], [16], 4, 2, 128, seed=6)
+        clean = c.run().double().cpu().numpy()
+        params = c.pool[1 if kind == "k" else 3]
+        params[c.table[0, at // 16], 1, at % 16, 2, 1] = np.nan
+        got = c.run().double().cpu().numpy()
+        want = clean.copy()
+        for i in range(16):
+            if 200 - 16 + i >= at:
+                want[i, 2:, :] = np.nan if kind == "k" else want[i, 2:, :]
+                want[i, 2:, 64:96] = np.nan
+        assert np.array_equal(np.isnan(got), np.isnan(want))
+        seen = ~np.isnan(want)
+        ref, tol = Call([200], [16], 4, 2, 128, seed=6).want()
+        assert (np.abs(got - ref)[seen] <= tol[seen]).all()
+
+
+def test_infinite_and_large_queries():
+    """A NaN or infinite query poisons its own rows alone; bf16 queries past fp16's range work."""
+    c = Call([100, 50], [4, 1], 4, 2, 64, dtype="bf16", seed=8)
+    q, *rest = c.device_args()
+    clean = paged_int4_attention(q, *rest)
+    q[1, 2, 5] = float("nan")
+    q[4, 0, 0] = float("inf")
+    got = paged_int4_attention(q, *rest)
+    assert got[1, 2].isnan().all() and got[4, 0].isnan().all()
+    hit = torch.zeros_like(got, dtype=torch.bool)
+    hit[1, 2] = hit[4, 0] = True
+    assert torch.equal(got[~hit], clean[~hit])
+    c = Call([60], [2], 4, 2, 64, dtype="bf16", scale=1e-7, seed=9)
+    c.q = rounded(c.q * 2.0 ** 20, "bf16")
+    c.check()
+    c.q, c.given_scale, c.scale = rounded(c.q * 2.0 ** -60, "bf16"), 2.0 ** 40, 2.0 ** 40
+    c.check()
+
+
+def test_the_same_page_in_several_sequences():
+    """A shared prefix: table rows that name the same pages."""
+    c = Call([100, 100, 64], [1, 1, 2], 4, 2, 64, seed=10)
+    c.table[1] = c.table[0]
+    c.table[2, :4] = c.table[0, :4]
+    c.check()
+
+
+def test_another_stream_and_graphs():
+    """On a side stream; captured twice, each replayed between eager calls on changed inputs."""
+    c = Call([3000, 700, 90], [1, 2, 1], 6, 2, 128, page=64, seed=12)
+    q, cache, table, lens, cu, max_q, max_k = c.device_args()
+    eager = paged_int4_attention(q, cache, table, lens, cu, max_q, max_k)
+    c.check(eager)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        other = paged_int4_attention(q, cache, table, lens, cu, max_q, max_k)
+    side.synchronize()
+    assert torch.equal(other, eager)
+    graphs = []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = paged_int4_attention(q, cache, table, lens, cu, max_q, max_k)
+        graphs.append((graph, out))
+    for step in range(4):
+        q.copy_(torch.randn(q.shape, generator=torch.Generator().manual_seed(step)).half())
+        lens.copy_(ints([3000 - 500 * step, 700 - step, 90 + 0 * step]))
+        want = paged_int4_attention(q, cache, table, lens, cu, max_q, max_k)
+        for graph, out in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(out, want) for _, out in graphs)
+
+
+def test_a_serving_step_in_a_graph():
+    """extend, store and attention together: prompts are admitted, then decode steps replay one graph;
+    every step against the definition, then the sequences leave."""
+    heads, hk, dim, page, pages, batch = 4, 2, 64, 16, 24, 3
+    tables = PageTables.empty(pages, batch, 6, page)
+    cache = PagedInt4Cache.empty(pages, hk, dim, page)
+    for t in (cache.k_codes, cache.v_codes):
+        t.fill_(255)
+    for t in (cache.k_params, cache.v_params):
+        t.fill_(float("nan"))
+    gen = torch.Generator().manual_seed(3)
+    history = [[np.zeros((0, hk, dim))] * 2 for _ in range(batch)]
+
+    def step(new, q, k, v, tokens):
+        plan = tables.extend(new, tokens)
+        store_int4(k, v, cache, plan.slots)
+        out = paged_int4_attention(q, cache, tables.block_table, tables.seq_lens, plan.cu_seqlens, tokens, 96)
+        return plan, out
+
+    def make(tokens):
+        return [torch.randn(tokens, h, dim, generator=gen).half().cuda() for h in (heads, hk, hk)]
+
+    def check(plan, out, new, q, k, v):
+        cu = plan.cu_seqlens.tolist()
+        for b in range(batch):
+            for j, x in ((0, k), (1, v)):
+                codes, params = P.quantise(x[cu[b]:cu[b + 1]].double().cpu().numpy())
+                history[b][j] = np.concatenate([history[b][j], P.dequantise(codes, params, dim)])
+        pool = [a.cpu().numpy() for a in (cache.k_codes, cache.k_params, cache.v_codes, cache.v_params)]
+        lens, table = tables.seq_lens.tolist(), tables.block_table.cpu().numpy()
+        assert lens == [len(h[0]) for h in history]
+        ref, mag, size = P.attention(q.double().cpu().numpy(), *pool, dim, table, lens, cu, max(new), 96, True, dim ** -0.5)
+        assert (np.abs(out.double().cpu().numpy() - ref) <= tolerance(ref, mag, size, dim, "fp16")).all()
+        got = load_int4(cache, tables.block_table, ints(np.concatenate([[0], np.cumsum(lens)]).tolist()), sum(lens))
+        for j in (0, 1):
+            assert np.array_equal(got[j].double().cpu().numpy(), np.concatenate([h[j] for h in history]))
+
+    new = [20, 33, 1]
+    q, k, v = make(sum(new))
+    plan, out = step(ints(new), q, k, v, sum(new))
+    check(plan, out, new, q, k, v)
+    one, (q, k, v) = ints([1] * batch), make(batch)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        plan, out = step(one, q, k, v, batch)
+    for _ in range(20):
+        for t, fresh in zip((q, k, v), make(batch)):
+            t.copy_(fresh)
+        graph.replay()
+        torch.cuda.synchronize()
+        check(plan, out, [1] * batch, q, k, v)
+    tables.truncate(ints([0] * batch))
+    assert int(tables.free_count) == pages and sorted(tables.free_pages.tolist()) == list(range(pages))
+    assert (tables.block_table == -1).all() and not tables.seq_lens.any()

@@ -15,7 +15,7 @@ from pathlib import Path
 import torch
 
 LIB_PATH = Path(__file__).resolve().parent / "libtilemix_hip.so"
-ABI_VERSION = 4
+ABI_VERSION = 5
 
 ROUTING_MIXED = 0
 ROUTING_FP16 = 1
@@ -104,6 +104,49 @@ class RotaryParams(ctypes.Structure):
     ]
 
 
+class Kv4RowsParams(ctypes.Structure):
+    """Mirror of ``tilemix_kv4_rows_params``."""
+
+    _fields_ = [
+        ("k_codes", _vp), ("k_params", _vp), ("v_codes", _vp), ("v_params", _vp), ("k", _vp), ("v", _vp),
+        ("slots", _vp), ("block_table", _vp), ("cu_seqlens", _vp),
+        ("stride_k_token", _i64), ("stride_k_head", _i64),
+        ("stride_v_token", _i64), ("stride_v_head", _i64),
+        ("stride_table", _i64), ("tokens", _i64),
+        ("pages", _i32), ("page_size", _i32), ("heads", _i32), ("head_dim", _i32),
+        ("batch", _i32), ("table_columns", _i32), ("dtype", _i32),
+    ]
+
+
+class Kv4AttnParams(ctypes.Structure):
+    """Mirror of ``tilemix_kv4_attn_params``."""
+
+    _fields_ = [
+        ("q", _vp), ("out", _vp), ("k_codes", _vp), ("k_params", _vp), ("v_codes", _vp), ("v_params", _vp),
+        ("block_table", _vp), ("seq_lens", _vp), ("cu_seqlens_q", _vp), ("workspace", _vp),
+        ("workspace_bytes", _i64),
+        ("stride_q_token", _i64), ("stride_q_head", _i64),
+        ("stride_o_token", _i64), ("stride_o_head", _i64),
+        ("stride_table", _i64), ("tokens_q", _i64),
+        ("sm_scale", _f32),
+        ("pages", _i32), ("page_size", _i32), ("heads_q", _i32), ("heads_k", _i32), ("head_dim", _i32),
+        ("batch", _i32), ("table_columns", _i32),
+        ("max_seqlen_q", _i32), ("max_seqlen_k", _i32),
+        ("causal", _i32), ("dtype", _i32),
+    ]
+
+
+class Kv4TablesParams(ctypes.Structure):
+    """Mirror of ``tilemix_kv4_tables_params``."""
+
+    _fields_ = [
+        ("block_table", _vp), ("seq_lens", _vp), ("free_pages", _vp), ("free_count", _vp), ("ticket", _vp),
+        ("lens", _vp), ("slots", _vp), ("positions", _vp), ("cu_seqlens", _vp), ("granted", _vp),
+        ("stride_table", _i64), ("tokens", _i64),
+        ("batch", _i32), ("table_columns", _i32), ("page_size", _i32), ("free_capacity", _i32),
+    ]
+
+
 EXPORTED_SYMBOLS = (
     "tilemix_quant_per_block_int8",
     "tilemix_quant_per_block_int8_many",
@@ -113,6 +156,12 @@ EXPORTED_SYMBOLS = (
     "tilemix_rms_norm_f16",
     "tilemix_rotary_f16",
     "tilemix_silu_mul_f16",
+    "tilemix_kv4_store",
+    "tilemix_kv4_load",
+    "tilemix_kv4_attn",
+    "tilemix_kv4_attn_workspace",
+    "tilemix_kv4_extend",
+    "tilemix_kv4_truncate",
     "tilemix_abi_version",
     "tilemix_params_size",
     "tilemix_last_error",
@@ -155,7 +204,8 @@ def load_library(path: os.PathLike | str | None = None) -> ctypes.CDLL:
             raise TileMixLibraryError(f"{lib_path} does not export {', '.join(missing)}; rebuild it")
         lib.tilemix_params_size.argtypes = [ctypes.c_int]
         lib.tilemix_params_size.restype = ctypes.c_int64
-        for which, struct in ((0, QuantParams), (1, AttnParams), (2, RmsNormParams), (3, RotaryParams)):
+        for which, struct in enumerate((QuantParams, AttnParams, RmsNormParams, RotaryParams, Kv4RowsParams,
+                                        Kv4AttnParams, Kv4TablesParams)):
             if lib.tilemix_params_size(which) != ctypes.sizeof(struct):
                 raise TileMixLibraryError(
                     f"{lib_path}: {struct.__name__} size {lib.tilemix_params_size(which)} != "
@@ -177,6 +227,13 @@ def load_library(path: os.PathLike | str | None = None) -> ctypes.CDLL:
         lib.tilemix_rotary_f16.restype = ctypes.c_int
         lib.tilemix_silu_mul_f16.argtypes = [_vp, _vp, _vp, _i64, _vp]
         lib.tilemix_silu_mul_f16.restype = ctypes.c_int
+        for name, struct in (("store", Kv4RowsParams), ("load", Kv4RowsParams), ("attn", Kv4AttnParams),
+                             ("extend", Kv4TablesParams), ("truncate", Kv4TablesParams)):
+            fn = getattr(lib, f"tilemix_kv4_{name}")
+            fn.argtypes = [ctypes.POINTER(struct), _vp]
+            fn.restype = ctypes.c_int
+        lib.tilemix_kv4_attn_workspace.argtypes = [ctypes.POINTER(Kv4AttnParams)]
+        lib.tilemix_kv4_attn_workspace.restype = ctypes.c_int64
         lib.tilemix_last_error.argtypes = []
         lib.tilemix_last_error.restype = ctypes.c_char_p
         if path is None:
@@ -193,6 +250,8 @@ def _check_host(module, lib: ctypes.CDLL) -> None:
     from .csrc.build import torch_id
     built = module.built_for() if hasattr(module, "built_for") else None
     now = (lib.tilemix_abi_version(), tuple(lib.tilemix_params_size(which) for which in range(4)), torch_id())
+    if built == now:  # the structs of the 4-bit cache, which a module of this version has
+        built, now = module.kv4_built_for(), tuple(lib.tilemix_params_size(which) for which in (4, 5, 6))
     if built != now:
         raise TileMixLibraryError(
             f"tilemix_amd/_host.so was built for {built}, loaded are {now} (ABI version, struct sizes, torch): "
@@ -218,6 +277,9 @@ def host():
             module.bind(*(ctypes.cast(fn, _vp).value for fn in (
                 lib.tilemix_quant_per_block_int8_many, lib.tilemix_attn_fwd, lib.tilemix_attn_fwd_uniform,
                 lib.tilemix_rms_norm_f16, lib.tilemix_rotary_f16, lib.tilemix_silu_mul_f16)))
+            module.kv4_bind(*(ctypes.cast(fn, _vp).value for fn in (
+                lib.tilemix_kv4_store, lib.tilemix_kv4_load, lib.tilemix_kv4_attn, lib.tilemix_kv4_attn_workspace,
+                lib.tilemix_kv4_extend, lib.tilemix_kv4_truncate, lib.tilemix_last_error)), TileMixLibraryError)
             _host = module
     return _host
 

@@ -4,7 +4,7 @@ Usage: python -m tilemix_amd.csrc.build   (or tilemix_amd.csrc.build.build())
 
 Every .hip file under this directory is compiled to an object in
 tilemix_amd/_build/ (in parallel) and linked into tilemix_amd/libtilemix_hip.so;
-host.cpp becomes the CPython extension module tilemix_amd/_host.so (the C++
+host.cpp and host_kv4.cpp become the CPython extension module tilemix_amd/_host.so (the C++
 compiler, against the installed torch).
 """
 from __future__ import annotations
@@ -84,7 +84,8 @@ def _host_command(out: Path) -> list[str]:
     return [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
             "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", f'-DTILEMIX_TORCH="{torch_id()}"',
             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-            *(arg for path in includes for arg in ("-isystem", str(path))), str(CSRC / "host.cpp"), "-o", str(out),
+            *(arg for path in includes for arg in ("-isystem", str(path))), str(CSRC / "host.cpp"),
+            str(CSRC / "host_kv4.cpp"), "-o", str(out),
             f"-L{root / 'lib'}", f"-Wl,-rpath,{root / 'lib'}", "-ltorch_python", "-ltorch_cpu", "-lc10_hip", "-lc10"]
 
 

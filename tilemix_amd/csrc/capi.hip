@@ -88,6 +88,54 @@ int tilemix_silu_mul_f16(const void* gate, const void* up, void* out, int64_t n,
   return tmx::launch_silu_mul(gate, up, out, n, static_cast<hipStream_t>(stream));
 }
 
+int tilemix_kv4_store(const tilemix_kv4_rows_params* p, void* stream) {
+  if (p == nullptr) {
+    tmx::set_error("tilemix_kv4_store: null params");
+    return TILEMIX_E_INVALID;
+  }
+  return tmx::launch_kv4_store(*p, static_cast<hipStream_t>(stream));
+}
+
+int tilemix_kv4_load(const tilemix_kv4_rows_params* p, void* stream) {
+  if (p == nullptr) {
+    tmx::set_error("tilemix_kv4_load: null params");
+    return TILEMIX_E_INVALID;
+  }
+  return tmx::launch_kv4_load(*p, static_cast<hipStream_t>(stream));
+}
+
+int tilemix_kv4_attn(const tilemix_kv4_attn_params* p, void* stream) {
+  if (p == nullptr) {
+    tmx::set_error("tilemix_kv4_attn: null params");
+    return TILEMIX_E_INVALID;
+  }
+  return tmx::launch_kv4_attn(*p, static_cast<hipStream_t>(stream));
+}
+
+int64_t tilemix_kv4_attn_workspace(const tilemix_kv4_attn_params* p) {
+  if (p == nullptr) {
+    tmx::set_error("tilemix_kv4_attn_workspace: null params");
+    return -1;
+  }
+  return tmx::kv4_attn_workspace(*p);
+}
+
+int tilemix_kv4_extend(const tilemix_kv4_tables_params* p, void* stream) {
+  if (p == nullptr) {
+    tmx::set_error("tilemix_kv4_extend: null params");
+    return TILEMIX_E_INVALID;
+  }
+  return tmx::launch_kv4_tables(*p, true, static_cast<hipStream_t>(stream));
+}
+
+int tilemix_kv4_truncate(const tilemix_kv4_tables_params* p, void* stream) {
+  if (p == nullptr) {
+    tmx::set_error("tilemix_kv4_truncate: null params");
+    return TILEMIX_E_INVALID;
+  }
+  return tmx::launch_kv4_tables(*p, false, static_cast<hipStream_t>(stream));
+}
+
 int tilemix_abi_version(void) { return TILEMIX_ABI_VERSION; }
 
 int64_t tilemix_params_size(int which) {
@@ -100,6 +148,12 @@ int64_t tilemix_params_size(int which) {
       return (int64_t)sizeof(tilemix_rmsnorm_params);
     case 3:
       return (int64_t)sizeof(tilemix_rotary_params);
+    case 4:
+      return (int64_t)sizeof(tilemix_kv4_rows_params);
+    case 5:
+      return (int64_t)sizeof(tilemix_kv4_attn_params);
+    case 6:
+      return (int64_t)sizeof(tilemix_kv4_tables_params);
     default:
       return -1;
   }

@@ -31,6 +31,11 @@ int launch_attn(const tilemix_attn_params& p, int uniform_seqlen, int32_t* dump_
 int launch_rmsnorm(const tilemix_rmsnorm_params& p, hipStream_t stream);
 int launch_rotary(const tilemix_rotary_params& p, hipStream_t stream);
 int launch_silu_mul(const void* gate, const void* up, void* out, int64_t n, hipStream_t stream);
+int launch_kv4_store(const tilemix_kv4_rows_params& p, hipStream_t stream);
+int launch_kv4_load(const tilemix_kv4_rows_params& p, hipStream_t stream);
+int launch_kv4_attn(const tilemix_kv4_attn_params& p, hipStream_t stream);
+int64_t kv4_attn_workspace(const tilemix_kv4_attn_params& p);
+int launch_kv4_tables(const tilemix_kv4_tables_params& p, bool extend, hipStream_t stream);
 
 // Exchange a value between lane l and lane l^32 of a wave64 and combine:
 // returns {value of this lane, value of the partner lane} as (lo, hi) pair

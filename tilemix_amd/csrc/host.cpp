@@ -26,6 +26,7 @@
 #include <cstdlib>
 #include <cstring>
 
+#include "host_kv4.h"
 #include "tilemix_hip.h"
 
 namespace {
@@ -590,6 +591,10 @@ PyMethodDef g_methods[] = {method<built_for>("built_for"),
                            method<bind>("bind"),     method<packed>("packed"),     method<dense>("dense"),
                            method<quantize>("quantize"),
                            method<rms_norm>("rms_norm"), method<rotary>("rotary"), method<silu_mul>("silu_mul"),
+                           method<kv4_bind>("kv4_bind"), method<kv4_built_for>("kv4_built_for"),
+                           method<kv4_check>("kv4_check"), method<kv4_store>("kv4_store"),
+                           method<kv4_load>("kv4_load"), method<kv4_attention>("kv4_attention"),
+                           method<kv4_extend>("kv4_extend"), method<kv4_truncate>("kv4_truncate"),
                            PyMethodDef{nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_host", nullptr, -1, g_methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -1,0 +1,681 @@
+// Attention over the paged 4-bit cache (format and arguments: include/tilemix_hip.h).
+//
+// A workgroup takes one (sequence, KV head), up to 16 RT of its query rows -- a row is a (query token,
+// query head of the group) pair -- and one split of the keys.  Its four waves take the split's
+// 64-key tiles in turn and join their running maxima, sums and outputs in LDS at the end; with
+// several splits the parts go to the workspace and kv4_join_kernel adds them up.
+//
+// The mathematics of a tile, in fp32 but for the operands of the matrix instructions:
+//   S^T = K Q^T          keys x rows, K's values fp16(n s + m) exactly as the cache defines them
+//   p = exp2(S^T c - M)  c = sm_scale log2(e), M the row's running maximum
+//   O^T += V^T P^T       channels x rows
+// p is rounded to fp16 for the second product (p <= 2^8, see kKv4Slack; relative error 2^-11,
+// as small as the output's own rounding), the row sum adds the unrounded p.
+#include "kv4_common.h"
+
+#include <algorithm>
+
+namespace tmx {
+
+namespace {
+
+constexpr int kTile = 64;  // keys
+constexpr int kWaves = 4;
+// The running maximum is raised when a row exceeds it by this much (in powers of two): most
+// tiles then leave the outputs unscaled.
+constexpr float kKv4Slack = 8.0f;
+constexpr float kNoKey = -1e30f;  // running maximum of a row without keys
+
+struct Kv4Args {
+  const void* q;
+  void* out;
+  const uint32_t* kc;
+  const uint32_t* kp;
+  const uint32_t* vc;
+  const uint32_t* vp;
+  const int32_t* table;
+  const int32_t* lens;
+  const int32_t* cu;
+  float* part;     // [item][split][row][channel] sums, unnormalised
+  float2* part_ml; // [item][split][row] maximum, sum
+  int64_t sq_t, sq_h, so_t, so_h, s_table, tokens;
+  float scale;
+  int pages, hq, hk, group, d, columns, max_q, max_k, causal, bf, q_vec, o_vec;
+  int row_blocks, splits, split_tiles;
+  FastDiv by_page, by_group, by_splits;
+};
+
+// One (sequence, KV head, block of query rows): its rows and keys.
+struct Kv4Item {
+  int b, h, rb;
+  int64_t start;  // first query token
+  int nq, rows;   // queries, rows of all its blocks
+  int len;        // keys
+  int limit0;     // keys that query 0 sees (may be <= 0)
+  int kmax;       // keys that the block's last row sees
+};
+
+__device__ __forceinline__ Kv4Item kv4_item(const Kv4Args& a, int b, int h, int rb, int block_rows) {
+  Kv4Item it;
+  it.b = b;
+  it.h = h;
+  it.rb = rb;
+  int64_t start = (int64_t)b * a.max_q;
+  int nq = a.max_q;
+  if (a.cu != nullptr) {
+    start = a.cu[b];
+    nq = a.cu[b + 1] - (int)start;
+  }
+  if (start < 0 || start > a.tokens) nq = 0;
+  nq = (int)min((int64_t)min(nq, a.max_q), a.tokens - start);
+  it.start = start;
+  it.nq = max(nq, 0);
+  it.rows = it.nq * a.group;
+  const int64_t room = min((int64_t)a.columns * a.by_page.d, (int64_t)a.max_k);
+  it.len = (int)min((int64_t)max(a.lens[b], 0), room);
+  it.limit0 = a.causal ? it.len - it.nq + 1 : it.len;
+  const int last = min(it.rows, (rb + 1) * block_rows) - 1;
+  it.kmax = a.causal ? it.limit0 + fast_div(max(last, 0), a.by_group) : it.len;
+  return it;
+}
+
+__device__ __forceinline__ float lanes16_max(float x) {
+  auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  const float2 h = swap_halves(x);
+  return fmaxf(h.x, h.y);
+}
+__device__ __forceinline__ float lanes16_sum(float x) {
+  auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  const float2 h = swap_halves(x);
+  return h.x + h.y;
+}
+__device__ __forceinline__ uint32_t lanes16_or(uint32_t x) {
+  auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+  x = r[0] | r[1];
+  auto s = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+  return s[0] | s[1];
+}
+
+// ---- lane layouts ---------------------------------------------------------------
+// Lane l = 16 g + i of a wave.  Matrix operands of 16x16x32: A holds row i, B column i, both the
+// k-slots 8 g .. 8 g + 7; the result holds column i and rows 4 g .. 4 g + 3.
+//  * QK: A = K.  Of a tile's four groups of 16 result rows, t = 0 .. 3, row i is key
+//    16 (i / 4) + 4 t + i % 4: result rows 4 g + e are then keys 16 g + 4 t + e, so a lane ends up with
+//    the 16 consecutive keys 16 g .. 16 g + 15 of query row i.  The slots of step s are the
+//    channels of word NG g + s of a row (word: eight channels), in the pairs of kv4_codes: a lane
+//    reads NG consecutive words of a key, whose group is theirs alone (NG = 3: one of two).
+//  * PV: A = V^T through ds_read_b64_tr_b4, which transposes a 16 x 16 block of codes in each 16 lanes:
+//    lane i gets channel i of the 16 rows that the lanes point at, here keys 16 g .. 16 g + 15.
+//    Word w of it are keys 16 g + 8 w .. + 7, in the pairs (0, 4), (1, 5) ..: the pairs
+//    (S[2 w][e], S[2 w + 1][e]) of the lane's own results, so P stays in registers.
+template <int NG>
+struct Kv4Tile {
+  static constexpr int kW = NG;              // words of a lane's part of a K or V row
+  static constexpr int kNP = NG == 3 ? 2 : 1;  // groups that these words can lie in
+  static constexpr int kStride = 16 * NG + 8;  // bytes of a V row in LDS: odd in 8-byte units, no bank conflicts
+  uint32_t k[4][kW], v[4][kW], kp[4][kNP], vp[NG];
+};
+
+// LDS of one wave: V codes, then the scales and minima [NG][64] each in the key order of the pairs.
+template <int NG>
+constexpr int kWaveLds = 64 * Kv4Tile<NG>::kStride + NG * 64 * 4;
+
+template <int NG, int RT>
+constexpr int kv4_lds_bytes() {
+  const int tiles = kWaves * kWaveLds<NG>, join = kWaves * 2 * NG * 64 * 16;  // one row tile at a time
+  return (tiles > join ? tiles : join) + kWaves * RT * 16 * 8;
+}
+
+template <int N>
+__device__ __forceinline__ void load_words(uint32_t (&to)[N], const uint32_t* from) {
+  if constexpr (N == 4) {
+    const u32x4 x = *reinterpret_cast<const u32x4*>(from);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) to[i] = x[i];
+  } else if constexpr (N == 2) {
+    const uint2 x = *reinterpret_cast<const uint2*>(from);
+    to[0] = x.x;
+    to[1] = x.y;
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) to[i] = from[i];
+  }
+}
+
+// The page of the lane's 16 keys 16 (i / 4) .. + 15 of a tile: -1 where there is none.
+__device__ __forceinline__ int page_of(const Kv4Args& a, const int32_t* table, int key, int kmax) {
+  if (key >= kmax) return -1;
+  const int id = table[fast_div(key, a.by_page)];
+  return id < a.pages ? id : -1;
+}
+
+template <int NG>
+__device__ __forceinline__ void load_tile(Kv4Tile<NG>& x, const Kv4Args& a, int h, int key, int page) {
+  const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
+  if (page < 0) {
+    x = Kv4Tile<NG>{};
+    return;
+  }
+  const int column = fast_div(key, a.by_page);
+  const int64_t row = ((int64_t)page * a.hk + h) * a.by_page.d + (key - column * a.by_page.d) + (i & 3);
+  const uint32_t* const kc = a.kc + row * (4 * NG) + NG * g;
+  const uint32_t* const vc = a.vc + row * (4 * NG) + NG * g;
+  const uint32_t* const kp = a.kp + row * NG;
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+    load_words(x.k[t], kc + t * (16 * NG));
+#pragma unroll
+    for (int j = 0; j < Kv4Tile<NG>::kNP; ++j) {
+      const int group = NG == 4 ? g : j == 0 ? NG * g / 4 : (NG * g + NG - 1) / 4;
+      x.kp[t][j] = kp[t * (4 * NG) + group];
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < 4; ++t) load_words(x.v[t], vc + t * (16 * NG));
+  load_words(x.vp, a.vp + (row + 4 * g) * NG);  // of key 16 (i / 4) + 4 g + i % 4
+}
+
+template <int NG, int RT>
+__global__ void __launch_bounds__(kWaves * 64, 2) kv4_attn_kernel(const Kv4Args a) {
+  using Tile = Kv4Tile<NG>;
+  constexpr int kCT = 2 * NG;  // tiles of 16 channels
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
+  const int rb = fast_div(blockIdx.x, a.by_splits), split = blockIdx.x - rb * a.splits;
+  const Kv4Item it = kv4_item(a, blockIdx.z, blockIdx.y, rb, 16 * RT);
+  const int row0 = rb * 16 * RT;
+  if (row0 >= it.rows) return;
+  const int tiles = it.kmax <= 0 ? 0 : (it.kmax + kTile - 1) / kTile;
+  const int first = split * a.split_tiles, last = min(tiles, first + a.split_tiles);
+  if (first >= last && split > 0) return;
+
+  // ---- queries: B operand of QK, rows 16 rt + i ----
+  f16x8 qf[RT][NG];
+  float scale[RT];
+  int limit[RT];
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    const int row = row0 + 16 * rt + i, token = fast_div(row, a.by_group), head = row - token * a.group;
+    const bool there = row < it.rows;
+    limit[rt] = a.causal ? it.limit0 + token : it.len;
+    scale[rt] = a.scale;
+    const int64_t at = (it.start + token) * a.sq_t + (it.h * a.group + head) * a.sq_h;
+    f32x8 x[NG];
+    float top = 0.0f;
+#pragma unroll
+    for (int s = 0; s < NG; ++s) {
+      const int c = 8 * (NG * g + s), n = there ? min(8, a.d - c) : 0;
+      x[s] = f32x8{};
+      if (a.bf) {
+        const bf16* const from = static_cast<const bf16*>(a.q) + at + c;
+        if (a.q_vec && n == 8) {
+          x[s] = __builtin_convertvector(*reinterpret_cast<const bf16x8*>(from), f32x8);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (e < n) x[s][e] = (float)from[e];
+        }
+      } else {
+        const f16* const from = static_cast<const f16*>(a.q) + at + c;
+        if (a.q_vec && n == 8) {
+          x[s] = __builtin_convertvector(*reinterpret_cast<const f16x8*>(from), f32x8);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (e < n) x[s][e] = (float)from[e];
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[s][e]));
+    }
+    // bf16 queries are held as fp16 times a power of two of their row: exact but for elements below
+    // 2^-14 of the row's largest, which lose no more than 2^-25 of that one.
+    if (a.bf) {
+      const int e = __builtin_amdgcn_frexp_expf(lanes16_max(top));
+      scale[rt] = ldexpf(scale[rt], e);
+#pragma unroll
+      for (int s = 0; s < NG; ++s)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[s][j] = ldexpf(x[s][j], -e);
+    }
+#pragma unroll
+    for (int s = 0; s < NG; ++s)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        qf[rt][s][2 * j] = (f16)x[s][j];
+        qf[rt][s][2 * j + 1] = (f16)x[s][j + 4];
+      }
+  }
+
+  f32x4 o[RT][kCT];
+  float top[RT], sum[RT];
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    top[rt] = kNoKey;
+    sum[rt] = 0.0f;
+#pragma unroll
+    for (int ct = 0; ct < kCT; ++ct) o[rt][ct] = f32x4{};
+  }
+
+  unsigned char* const lds_v = smem + wave * kWaveLds<NG>;
+  f16* const lds_s = reinterpret_cast<f16*>(lds_v + 64 * Tile::kStride);
+  f16* const lds_m = lds_s + NG * 64;
+  const int32_t* const table = a.table + it.b * a.s_table;
+  const int all_see = it.limit0 + (a.causal ? fast_div(row0, a.by_group) : 0);  // keys that every row sees
+  const int key_i = 16 * (i >> 2);  // first of the lane's 16 keys of a tile
+  // position of key 4 g + i % 4 of 16 in the pairs' order (0, 4), (1, 5), (2, 6), (3, 7), (8, 12) ..
+  const int p_at = key_i + 8 * (g >> 1) + 2 * (i & 3) + (g & 1);
+
+  Tile x;
+  int tile = first + wave;
+  int page = page_of(a, table, tile * kTile + key_i, min(it.kmax, last * kTile));
+  int next = page_of(a, table, (tile + kWaves) * kTile + key_i, min(it.kmax, last * kTile));
+  load_tile(x, a, it.h, tile * kTile + key_i, page);
+  for (; tile < last; tile += kWaves) {
+    const int key0 = tile * kTile;
+    const uint64_t pages = __ballot(page >= 0);
+    // keys behind the last one that any row sees may hold anything: they become zeros
+    {
+      const bool gone = key0 + key_i + 4 * g + (i & 3) >= it.kmax;
+#pragma unroll
+      for (int j = 0; j < NG; ++j) x.vp[j] = gone ? 0u : x.vp[j];
+    }
+    uint32_t broken = 0;  // groups of the lane's key whose values are not finite: zeros here, see below
+#pragma unroll
+    for (int j = 0; j < NG; ++j)
+      if (kv4_not_finite(x.vp[j])) {
+        broken |= 1u << j;
+        x.vp[j] = 0;
+      }
+    // ---- V codes and parameters to LDS ----
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      uint32_t* const to =
+          reinterpret_cast<uint32_t*>(lds_v + (key_i + 4 * t + (i & 3)) * Tile::kStride) + Tile::kW * g;
+      if constexpr (NG == 4) {
+        *reinterpret_cast<uint2*>(to) = make_uint2(x.v[t][0], x.v[t][1]);
+        *reinterpret_cast<uint2*>(to + 2) = make_uint2(x.v[t][2], x.v[t][3]);
+      } else if constexpr (NG == 2) {
+        *reinterpret_cast<uint2*>(to) = make_uint2(x.v[t][0], x.v[t][1]);
+      } else {
+#pragma unroll
+        for (int s = 0; s < NG; ++s) to[s] = x.v[t][s];
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < NG; ++j) {
+      const f16x2 sm = __builtin_bit_cast(f16x2, x.vp[j]);
+      lds_s[j * 64 + p_at] = sm[0];
+      lds_m[j * 64 + p_at] = sm[1];
+    }
+    // ---- S^T = K Q^T ----
+    f32x4 acc[RT][4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) acc[rt][t] = f32x4{};
+#pragma unroll
+      for (int s = 0; s < NG; ++s) {
+        const uint32_t p = NG == 3 && (NG * g + s) / 4 != NG * g / 4 ? x.kp[t][Tile::kNP - 1] : x.kp[t][0];
+        const f16x2 sm = __builtin_bit_cast(f16x2, p), sc = {sm[0], sm[0]}, mn = {sm[1], sm[1]};
+        f16x2 n[4];
+        kv4_codes(x.k[t][s], n);
+        f16x8 kf;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const f16x2 v = kv4_fma(n[j], sc, mn);
+          kf[2 * j] = v[0];
+          kf[2 * j + 1] = v[1];
+        }
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+          acc[rt][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[rt][s], acc[rt][t], 0, 0, 0);
+      }
+    }
+    // ---- the next tile is on its way while this one goes on ----
+    page = next;
+    load_tile(x, a, it.h, key0 + kWaves * kTile + key_i, page);
+    next = page_of(a, table, key0 + 2 * kWaves * kTile + key_i, min(it.kmax, last * kTile));
+    // ---- softmax ----
+    const bool masked = key0 + kTile > all_see || pages != ~0ull;
+    f16x8 pf[RT][2];
+    const int mine = key0 + 16 * g;  // the lane's 16 keys
+    const bool mine_there = (pages >> (4 * g)) & 1;
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      // the scale may be negative: it comes before the maximum
+#pragma unroll
+      for (int t = 0; t < 4; ++t) acc[rt][t] *= scale[rt];
+      if (masked) {
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (!mine_there || mine + 4 * t + e >= limit[rt]) acc[rt][t][e] = -__builtin_inff();
+      }
+      float hi = -__builtin_inff();
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) hi = fmaxf(hi, acc[rt][t][e]);
+      hi = lanes16_max(hi);
+      if (__any(hi > top[rt] + kKv4Slack)) {
+        const float up = fmaxf(hi, top[rt]), down = __builtin_amdgcn_exp2f(top[rt] - up);
+        top[rt] = up;
+        sum[rt] *= down;
+#pragma unroll
+        for (int ct = 0; ct < kCT; ++ct) o[rt][ct] *= down;
+      }
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          acc[rt][t][e] = __builtin_amdgcn_exp2f(acc[rt][t][e] - top[rt]);
+          sum[rt] += acc[rt][t][e];
+        }
+#pragma unroll
+      for (int w = 0; w < 2; ++w)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          pf[rt][w][2 * e] = (f16)acc[rt][2 * w][e];
+          pf[rt][w][2 * e + 1] = (f16)acc[rt][2 * w + 1][e];
+        }
+    }
+    // ---- O^T += V^T P^T ----
+    const unsigned char* const v_at = lds_v + (16 * g + i) * Tile::kStride;
+#pragma unroll
+    for (int j = 0; j < NG; ++j) {
+      f16x2 sc[8], mn[8];
+#pragma unroll
+      for (int w = 0; w < 2; ++w) {
+        const f16x8 s8 = *reinterpret_cast<const f16x8*>(lds_s + j * 64 + 16 * g + 8 * w);
+        const f16x8 m8 = *reinterpret_cast<const f16x8*>(lds_m + j * 64 + 16 * g + 8 * w);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          sc[4 * w + e] = f16x2{s8[2 * e], s8[2 * e + 1]};
+          mn[4 * w + e] = f16x2{m8[2 * e], m8[2 * e + 1]};
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const int ct = 2 * j + c;
+        const i32x2 words = __builtin_amdgcn_ds_read_tr4_b64_v2i32(
+            (__attribute__((address_space(3))) i32x2*)(v_at + 8 * ct));
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+          f16x2 n[4];
+          kv4_codes((uint32_t)words[w], n);
+          f16x8 vf;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const f16x2 v = kv4_fma(n[e], sc[4 * w + e], mn[4 * w + e]);
+            vf[2 * e] = v[0];
+            vf[2 * e + 1] = v[1];
+          }
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt)
+            o[rt][ct] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[rt][w], o[rt][ct], 0, 0, 0);
+        }
+      }
+    }
+    // Values that are not finite (a NaN was stored): the rows that see the key get a NaN in the
+    // group's channels, the others must not (0 times NaN would be one).
+    if (__any(broken != 0)) {
+      uint32_t seen[RT] = {};
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+#pragma unroll
+        for (int k = 0; k < 16; ++k) {
+          // key 16 g + k is held by the lane 16 (k / 4) + 4 g + k % 4
+          const uint32_t bad = __shfl(broken, 16 * (k >> 2) + 4 * g + (k & 3), 64);
+          if (mine + k < limit[rt]) seen[rt] |= bad;
+        }
+        seen[rt] = lanes16_or(seen[rt]);
+#pragma unroll
+        for (int ct = 0; ct < kCT; ++ct)
+          if ((seen[rt] >> (ct >> 1)) & 1) o[rt][ct] = f32x4{} + __builtin_nanf("");
+      }
+    }
+  }
+
+  // ---- the four waves' parts ----
+  float2* const lds_ml = reinterpret_cast<float2*>(smem + kv4_lds_bytes<NG, RT>() - kWaves * RT * 16 * 8);
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    sum[rt] = lanes16_sum(sum[rt]);
+    if (g == 0) lds_ml[(wave * RT + rt) * 16 + i] = make_float2(top[rt], sum[rt]);
+  }
+  const int item = ((it.b * a.hk + it.h) * a.row_blocks + rb) * a.splits + split;
+  f32x4* const lds_o = reinterpret_cast<f32x4*>(smem);
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    __syncthreads();  // the tiles' LDS, or the row tile before, is no longer read
+    float all_top = kNoKey, all_sum = 0.0f;
+    float2 ml[kWaves];
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      ml[w] = lds_ml[(w * RT + rt) * 16 + i];
+      all_top = fmaxf(all_top, ml[w].x);
+    }
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) all_sum += ml[w].y * __builtin_amdgcn_exp2f(ml[w].x - all_top);
+    const float down = __builtin_amdgcn_exp2f(top[rt] - all_top);
+#pragma unroll
+    for (int ct = 0; ct < kCT; ++ct) lds_o[(wave * kCT + ct) * 64 + lane] = o[rt][ct] * down;
+    __syncthreads();
+    const int row = row0 + 16 * rt + i, token = fast_div(row, a.by_group), head = row - token * a.group;
+    if (row < it.rows) {
+      if (a.splits > 1 && wave == 0 && g == 0)
+        a.part_ml[(int64_t)item * (16 * RT) + 16 * rt + i] = make_float2(all_top, all_sum);
+      const float norm = all_sum == 0.0f ? 0.0f : 1.0f / all_sum;
+      for (int ct = wave; ct < kCT; ct += kWaves) {
+        f32x4 r = lds_o[ct * 64 + lane];
+#pragma unroll
+        for (int w = 1; w < kWaves; ++w) r += lds_o[(w * kCT + ct) * 64 + lane];
+        const int c = 16 * ct + 4 * g;
+        if (a.splits > 1) {
+          *reinterpret_cast<f32x4*>(a.part + ((int64_t)item * (16 * RT) + 16 * rt + i) * (32 * NG) + c) = r;
+          continue;
+        }
+        r *= norm;
+        const int64_t at = (it.start + token) * a.so_t + (it.h * a.group + head) * a.so_h + c;
+        if (a.bf) {
+          bf16* const to = static_cast<bf16*>(a.out) + at;
+          const bf16x4 v = __builtin_convertvector(r, bf16x4);
+          if (a.o_vec && c + 4 <= a.d) *reinterpret_cast<bf16x4*>(to) = v;
+          else
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (c + e < a.d) to[e] = v[e];
+        } else {
+          f16* const to = static_cast<f16*>(a.out) + at;
+          const f16x4 v = __builtin_convertvector(r, f16x4);
+          if (a.o_vec && c + 4 <= a.d) *reinterpret_cast<f16x4*>(to) = v;
+          else
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (c + e < a.d) to[e] = v[e];
+        }
+      }
+    }
+  }
+}
+
+// Adds up the splits of a row: one thread per four channels.
+template <int NG>
+__global__ void __launch_bounds__(256) kv4_join_kernel(const Kv4Args a, int block_rows) {
+  constexpr int kLanes = 8 * NG, kRows = 256 / kLanes;
+  const int r = threadIdx.x / kLanes, c = 4 * (threadIdx.x - r * kLanes);
+  const int groups = (block_rows + kRows - 1) / kRows, rb = blockIdx.x / groups;
+  const int in_block = (blockIdx.x - rb * groups) * kRows + r;
+  const Kv4Item it = kv4_item(a, blockIdx.z, blockIdx.y, rb, block_rows);
+  const int row = rb * block_rows + in_block;
+  if (r >= kRows || in_block >= block_rows || row >= it.rows || c >= a.d) return;
+  const int tiles = it.kmax <= 0 ? 0 : (it.kmax + kTile - 1) / kTile;
+  const int parts = max(1, (tiles + a.split_tiles - 1) / a.split_tiles);
+  const int64_t first =
+      (int64_t)((it.b * a.hk + it.h) * a.row_blocks + rb) * a.splits * block_rows + in_block;
+  float top = kNoKey;
+  for (int s = 0; s < parts; ++s) top = fmaxf(top, a.part_ml[first + (int64_t)s * block_rows].x);
+  f32x4 o = {};
+  float sum = 0.0f;
+  for (int s = 0; s < parts; ++s) {
+    const int64_t at = first + (int64_t)s * block_rows;
+    const float2 ml = a.part_ml[at];
+    const float down = __builtin_amdgcn_exp2f(ml.x - top);
+    sum += ml.y * down;
+    o += *reinterpret_cast<const f32x4*>(a.part + at * (32 * NG) + c) * down;
+  }
+  o *= sum == 0.0f ? 0.0f : 1.0f / sum;
+  const int token = fast_div(row, a.by_group), head = row - token * a.group;
+  const int64_t at = (it.start + token) * a.so_t + (it.h * a.group + head) * a.so_h + c;
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (c + e < a.d) {
+      if (a.bf) static_cast<bf16*>(a.out)[at + e] = (bf16)o[e];
+      else static_cast<f16*>(a.out)[at + e] = (f16)o[e];
+    }
+}
+
+struct Plan {
+  int rt, row_blocks, splits, split_tiles;
+  int64_t bytes;
+};
+
+bool make_plan(const char* what, const tilemix_kv4_attn_params& p, Plan& plan) {
+  if (!kv4_pool_ok(what, p.k_codes, p.k_params, p.v_codes, p.v_params, p.pages, p.page_size, p.heads_k, p.head_dim,
+                   p.dtype))
+    return false;
+  if (p.heads_q <= 0 || p.heads_q % p.heads_k != 0 || p.batch < 0 || p.batch > 65535 || p.table_columns < 0 ||
+      p.max_seqlen_q < 0 || p.max_seqlen_k < 0 || p.tokens_q < 0 || p.tokens_q > INT32_MAX) {
+    set_error("%s: invalid sizes (heads %d/%d, batch %d, table_columns %d, max_seqlen %d/%d, %lld queries)", what,
+              p.heads_q, p.heads_k, p.batch, p.table_columns, p.max_seqlen_q, p.max_seqlen_k, (long long)p.tokens_q);
+    return false;
+  }
+  const int64_t rows = (int64_t)p.max_seqlen_q * (p.heads_q / p.heads_k);
+  plan.rt = rows <= 16 ? 1 : 2;
+  const int64_t blocks = (rows + 16 * plan.rt - 1) / (16 * plan.rt);
+  const int64_t keys = std::min<int64_t>(p.max_seqlen_k, (int64_t)p.table_columns * p.page_size);
+  const int64_t tiles = std::max<int64_t>((keys + kTile - 1) / kTile, 1);
+  const int64_t items = std::max<int64_t>(blocks * p.heads_k * p.batch, 1);
+  const int64_t wanted = std::max<int64_t>(1, (int64_t)1024 / items);
+  int64_t split_tiles = (tiles + wanted - 1) / wanted;
+  split_tiles = (split_tiles + kWaves - 1) / kWaves * kWaves;
+  const int64_t splits = (tiles + split_tiles - 1) / split_tiles;
+  const int64_t grid = blocks * splits;
+  if (rows > INT32_MAX || grid > (1 << 24) - 1 || items * splits > INT32_MAX / 64) {
+    set_error("%s: too many queries for one call (%lld rows a sequence, batch %d)", what, (long long)rows, p.batch);
+    return false;
+  }
+  plan.row_blocks = (int)blocks;
+  plan.splits = (int)splits;
+  plan.split_tiles = (int)split_tiles;
+  const int width = (p.head_dim + kKv4Group - 1) / kKv4Group * kKv4Group;
+  plan.bytes = splits > 1 ? items * splits * 16 * plan.rt * (width * 4 + 8) : 0;
+  return true;
+}
+
+template <int NG, int RT>
+void launch_kv4(const Kv4Args& a, int batch, hipStream_t stream) {
+  constexpr int lds = kv4_lds_bytes<NG, RT>();
+  hipLaunchKernelGGL((kv4_attn_kernel<NG, RT>), dim3((unsigned)(a.row_blocks * a.splits), a.hk, batch),
+                     dim3(kWaves * 64), lds, stream, a);
+  if (a.splits > 1) {
+    constexpr int rows = 256 / (8 * NG);
+    hipLaunchKernelGGL((kv4_join_kernel<NG>), dim3((unsigned)(a.row_blocks * ((16 * RT + rows - 1) / rows)), a.hk, batch),
+                       dim3(256), 0, stream, a, 16 * RT);
+  }
+}
+
+template <int NG>
+void launch_kv4(const Kv4Args& a, int rt, int batch, hipStream_t stream) {
+  if (rt == 1) launch_kv4<NG, 1>(a, batch, stream);
+  else launch_kv4<NG, 2>(a, batch, stream);
+}
+
+}  // namespace
+
+int64_t kv4_attn_workspace(const tilemix_kv4_attn_params& p) {
+  Plan plan;
+  return make_plan("tilemix_kv4_attn_workspace", p, plan) ? plan.bytes : -1;
+}
+
+int launch_kv4_attn(const tilemix_kv4_attn_params& p, hipStream_t stream) {
+  const char* const what = "tilemix_kv4_attn";
+  Plan plan;
+  if (!make_plan(what, p, plan)) return TILEMIX_E_INVALID;
+  if (p.batch == 0 || p.tokens_q == 0 || p.max_seqlen_q == 0) return TILEMIX_OK;
+  if (p.q == nullptr || p.out == nullptr || p.seq_lens == nullptr ||
+      (p.block_table == nullptr && p.table_columns > 0)) {
+    set_error("%s: null pointer", what);
+    return TILEMIX_E_INVALID;
+  }
+  if (plan.bytes > 0 && (p.workspace == nullptr || p.workspace_bytes < plan.bytes ||
+                         (reinterpret_cast<uintptr_t>(p.workspace) & 15) != 0)) {
+    set_error("%s: needs %lld bytes of 16-byte aligned workspace, got %lld", what, (long long)plan.bytes,
+              (long long)p.workspace_bytes);
+    return TILEMIX_E_INVALID;
+  }
+  const int width = (p.head_dim + kKv4Group - 1) / kKv4Group * kKv4Group;
+  Kv4Args a{};
+  a.q = p.q;
+  a.out = p.out;
+  a.kc = static_cast<const uint32_t*>(p.k_codes);
+  a.kp = static_cast<const uint32_t*>(p.k_params);
+  a.vc = static_cast<const uint32_t*>(p.v_codes);
+  a.vp = static_cast<const uint32_t*>(p.v_params);
+  a.table = p.block_table;
+  a.lens = p.seq_lens;
+  a.cu = p.cu_seqlens_q;
+  a.part = static_cast<float*>(p.workspace);
+  const int64_t parts = (int64_t)p.batch * p.heads_k * plan.row_blocks * plan.splits * 16 * plan.rt;
+  if (plan.bytes > 0) a.part_ml = reinterpret_cast<float2*>(a.part + parts * width);
+  a.sq_t = p.stride_q_token;
+  a.sq_h = p.stride_q_head;
+  a.so_t = p.stride_o_token;
+  a.so_h = p.stride_o_head;
+  a.s_table = p.stride_table;
+  a.tokens = p.tokens_q;
+  a.scale = p.sm_scale * kLog2eF32;
+  a.pages = p.pages;
+  a.hq = p.heads_q;
+  a.hk = p.heads_k;
+  a.group = p.heads_q / p.heads_k;
+  a.d = p.head_dim;
+  a.columns = p.table_columns;
+  a.max_q = p.max_seqlen_q;
+  a.max_k = p.max_seqlen_k;
+  a.causal = p.causal;
+  a.bf = p.dtype;
+  a.q_vec = (reinterpret_cast<uintptr_t>(p.q) & 15) == 0 && ((p.stride_q_token | p.stride_q_head) & 7) == 0;
+  a.o_vec = (reinterpret_cast<uintptr_t>(p.out) & 7) == 0 && ((p.stride_o_token | p.stride_o_head) & 3) == 0;
+  a.row_blocks = plan.row_blocks;
+  a.splits = plan.splits;
+  a.split_tiles = plan.split_tiles;
+  a.by_page = make_fast_div(p.page_size);
+  a.by_group = make_fast_div(a.group);
+  a.by_splits = make_fast_div(a.splits);
+  switch (width / kKv4Group) {
+    case 1:
+      launch_kv4<1>(a, plan.rt, p.batch, stream);
+      break;
+    case 2:
+      launch_kv4<2>(a, plan.rt, p.batch, stream);
+      break;
+    case 3:
+      launch_kv4<3>(a, plan.rt, p.batch, stream);
+      break;
+    default:
+      launch_kv4<4>(a, plan.rt, p.batch, stream);
+  }
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) {
+    set_error("%s: launch failed: %s", what, hipGetErrorString(e));
+    return TILEMIX_E_LAUNCH;
+  }
+  return TILEMIX_OK;
+}
+
+}  // namespace tmx

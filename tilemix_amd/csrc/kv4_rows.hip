@@ -1,0 +1,244 @@
+// Rows of K and V into the paged 4-bit cache and back (format: include/tilemix_hip.h).
+// Both are streaming kernels: at head_dim 128 a row is 256 bytes of values and 80 of codes
+// and parameters.
+#include "kv4_common.h"
+
+#include <algorithm>
+
+namespace tmx {
+
+bool kv4_pool_ok(const char* what, const void* kc, const void* kp, const void* vc, const void* vp, int pages,
+                 int page_size, int heads, int head_dim, int dtype) {
+  const uintptr_t codes = reinterpret_cast<uintptr_t>(kc) | reinterpret_cast<uintptr_t>(vc);
+  const uintptr_t params = reinterpret_cast<uintptr_t>(kp) | reinterpret_cast<uintptr_t>(vp);
+  if (kc == nullptr || kp == nullptr || vc == nullptr || vp == nullptr || (codes & 15) != 0 || (params & 3) != 0) {
+    set_error("%s: null or misaligned cache pointer", what);
+    return false;
+  }
+  if (pages <= 0 || page_size <= 0 || page_size % 16 != 0 || heads <= 0 || heads > 65535 || head_dim <= 0 ||
+      head_dim > 128 || (dtype != 0 && dtype != 1)) {
+    set_error("%s: invalid cache (pages %d, page_size %d, heads %d, head_dim %d, dtype %d)", what, pages, page_size,
+              heads, head_dim, dtype);
+    return false;
+  }
+  return true;
+}
+
+namespace {
+
+struct RowsArgs {
+  uint32_t* codes[2];   // K, V
+  uint32_t* params[2];
+  void* x[2];
+  const int64_t* slots;
+  const int32_t* table;
+  const int32_t* cu;
+  int64_t st[2], sh[2], s_table, tokens;
+  int pages, heads, d, batch, columns, vec;
+  FastDiv by_page;
+};
+
+// Thread = one word (eight channels) of a row: 4 NG threads a row, so that a wave reads
+// whole rows in 16-byte pieces and the four lanes of a group find its range among them.
+template <int NG>
+struct RowSplit {
+  static constexpr int kWords = 4 * NG;
+  static constexpr int kRows = 256 / kWords;  // of a workgroup (NG = 3: the last four threads idle)
+};
+
+__device__ __forceinline__ float quad_xor1(float x) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x), 0xb1, 0xf, 0xf, true));
+}
+__device__ __forceinline__ float quad_xor2(float x) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x), 0x4e, 0xf, 0xf, true));
+}
+
+template <typename T>
+__device__ __forceinline__ f32x8 read8(const T* x, int count, bool vec) {
+  typedef T T8 __attribute__((ext_vector_type(8)));
+  if (vec && count >= 8) return __builtin_convertvector(*reinterpret_cast<const T8*>(x), f32x8);
+  f32x8 v = {};
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    if (e < count) v[e] = (float)x[e];
+  return v;
+}
+
+template <int NG, typename T>
+__global__ void __launch_bounds__(256) kv4_store_kernel(const RowsArgs a) {
+  using S = RowSplit<NG>;
+  const int r = threadIdx.x / S::kWords, w = threadIdx.x - r * S::kWords, h = blockIdx.y, z = blockIdx.z;
+  const int64_t t = (int64_t)blockIdx.x * S::kRows + r;
+  if (r >= S::kRows || t >= a.tokens) return;
+  const int64_t slot = a.slots[t];
+  if (slot < 0 || slot >= (int64_t)a.pages * a.by_page.d) return;
+  const int there = min(8, a.d - 8 * w);  // channels of this word
+  const T* x = static_cast<const T*>(a.x[z]) + t * a.st[z] + h * a.sh[z] + 8 * w;
+  f32x8 v = read8(x, there, a.vec);
+  float lo = __builtin_inff(), hi = -__builtin_inff();
+  bool nan = false;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    nan |= e < there && v[e] != v[e];
+    v[e] = fminf(fmaxf(v[e], -kKv4Limit), kKv4Limit);
+    if (e < there) {
+      lo = fminf(lo, v[e]);
+      hi = fmaxf(hi, v[e]);
+    }
+  }
+  // (the four lanes of a group are in or out together: rows of four words each group)
+  lo = fminf(lo, quad_xor1(lo));
+  hi = fmaxf(hi, quad_xor1(hi));
+  lo = fminf(lo, quad_xor2(lo));
+  hi = fmaxf(hi, quad_xor2(hi));
+  float bad = nan ? 1.0f : 0.0f;
+  bad = fmaxf(bad, quad_xor1(bad));
+  bad = fmaxf(bad, quad_xor2(bad));
+  f16 s = (f16)((hi - lo) / 15.0f), m = (f16)lo;
+  if (bad != 0.0f) {
+    s = (f16)0.0f;
+    m = (f16)__builtin_nanf("");
+  }
+  const float step = (float)s, least = (float)m;
+  uint32_t word = 0;
+  if (step > 0.0f) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float n = fminf(fmaxf(rintf((v[e] - least) / step), 0.0f), 15.0f);
+      if (e < there) word |= (uint32_t)n << (4 * e);
+    }
+  }
+  const int page = (int)(slot / a.by_page.d), at = (int)(slot - (int64_t)page * a.by_page.d);
+  const int64_t row = ((int64_t)page * a.heads + h) * a.by_page.d + at;
+  a.codes[z][row * S::kWords + w] = word;
+  if ((w & 3) == 0)
+    a.params[z][row * NG + (w >> 2)] =
+        (uint32_t)__builtin_bit_cast(uint16_t, s) | (uint32_t)__builtin_bit_cast(uint16_t, m) << 16;
+}
+
+template <int NG, typename T>
+__global__ void __launch_bounds__(256) kv4_load_kernel(const RowsArgs a) {
+  using S = RowSplit<NG>;
+  typedef T T8 __attribute__((ext_vector_type(8)));
+  const int r = threadIdx.x / S::kWords, w = threadIdx.x - r * S::kWords, h = blockIdx.y, z = blockIdx.z;
+  const int64_t t0 = (int64_t)blockIdx.x * S::kRows, t = t0 + r;
+  // The sequence that ends behind the workgroup's first row: entries 1 .. batch - 1 of cu at or before it.
+  int b = 0;
+  for (int i = 1 + (threadIdx.x & 63); i - (int)(threadIdx.x & 63) < a.batch; i += 64)
+    b += __popcll(__ballot(i < a.batch && a.cu[i] <= t0));
+  if (r >= S::kRows || t >= a.tokens) return;
+  while (b + 1 < a.batch && a.cu[b + 1] <= t) ++b;
+  const int64_t start = a.cu[b];
+  int64_t row = -1;
+  if (t >= start && t < a.cu[b + 1]) {
+    const int at = (int)(t - start), column = fast_div(at, a.by_page);
+    const int page = column < a.columns ? a.table[b * a.s_table + column] : -1;
+    if (page >= 0 && page < a.pages) row = ((int64_t)page * a.heads + h) * a.by_page.d + at - column * a.by_page.d;
+  }
+  f16x2 v[4] = {};
+  if (row >= 0) {
+    const uint32_t p = a.params[z][row * NG + (w >> 2)];
+    const f16x2 sm = __builtin_bit_cast(f16x2, p), s = {sm[0], sm[0]}, m = {sm[1], sm[1]};
+    kv4_codes(a.codes[z][row * S::kWords + w], v);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = kv4_fma(v[i], s, m);
+  }
+  T8 out;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    out[i] = (T)(float)v[i][0];
+    out[i + 4] = (T)(float)v[i][1];
+  }
+  T* x = static_cast<T*>(a.x[z]) + t * a.st[z] + h * a.sh[z] + 8 * w;
+  const int there = min(8, a.d - 8 * w);
+  if (a.vec && there == 8) {
+    *reinterpret_cast<T8*>(x) = out;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e < there) x[e] = out[e];
+  }
+}
+
+template <int NG>
+void launch_rows(const RowsArgs& a, bool store, bool bf, hipStream_t stream) {
+  const dim3 grid((unsigned)((a.tokens + RowSplit<NG>::kRows - 1) / RowSplit<NG>::kRows), a.heads, 2), block(256);
+  if (store && bf) hipLaunchKernelGGL((kv4_store_kernel<NG, bf16>), grid, block, 0, stream, a);
+  else if (store) hipLaunchKernelGGL((kv4_store_kernel<NG, f16>), grid, block, 0, stream, a);
+  else if (bf) hipLaunchKernelGGL((kv4_load_kernel<NG, bf16>), grid, block, 0, stream, a);
+  else hipLaunchKernelGGL((kv4_load_kernel<NG, f16>), grid, block, 0, stream, a);
+}
+
+int run_rows(const char* what, const tilemix_kv4_rows_params& p, bool store, hipStream_t stream) {
+  if (!kv4_pool_ok(what, p.k_codes, p.k_params, p.v_codes, p.v_params, p.pages, p.page_size, p.heads, p.head_dim,
+                   p.dtype))
+    return TILEMIX_E_INVALID;
+  // The grid has at most 2^24 - 1 workgroups along x (HIP takes fewer than 2^32 threads); the fewest
+  // rows of one are 16.
+  if (p.tokens < 0 || p.tokens > (int64_t)16 * ((1 << 24) - 1)) {
+    set_error("%s: %lld rows in one call", what, (long long)p.tokens);
+    return TILEMIX_E_INVALID;
+  }
+  if (p.tokens == 0) return TILEMIX_OK;
+  if (p.k == nullptr || p.v == nullptr || (store && p.slots == nullptr) ||
+      (!store && (p.cu_seqlens == nullptr || p.batch <= 0 || p.table_columns < 0 ||
+                  (p.block_table == nullptr && p.table_columns > 0)))) {
+    set_error("%s: null pointer or no sequence", what);
+    return TILEMIX_E_INVALID;
+  }
+  RowsArgs a{};
+  void* const codes[2] = {p.k_codes, p.v_codes};
+  void* const params[2] = {p.k_params, p.v_params};
+  void* const x[2] = {p.k, p.v};
+  const int64_t st[2] = {p.stride_k_token, p.stride_v_token}, sh[2] = {p.stride_k_head, p.stride_v_head};
+  a.vec = 1;
+  for (int i = 0; i < 2; ++i) {
+    a.codes[i] = static_cast<uint32_t*>(codes[i]);
+    a.params[i] = static_cast<uint32_t*>(params[i]);
+    a.x[i] = x[i];
+    a.st[i] = st[i];
+    a.sh[i] = sh[i];
+    if ((reinterpret_cast<uintptr_t>(x[i]) & 15) != 0 || ((st[i] | sh[i]) & 7) != 0) a.vec = 0;
+  }
+  a.slots = p.slots;
+  a.table = p.block_table;
+  a.cu = p.cu_seqlens;
+  a.s_table = p.stride_table;
+  a.tokens = p.tokens;
+  a.pages = p.pages;
+  a.heads = p.heads;
+  a.d = p.head_dim;
+  a.batch = p.batch;
+  a.columns = p.table_columns;
+  a.by_page = make_fast_div(p.page_size);
+  switch ((p.head_dim + kKv4Group - 1) / kKv4Group) {
+    case 1:
+      launch_rows<1>(a, store, p.dtype == 1, stream);
+      break;
+    case 2:
+      launch_rows<2>(a, store, p.dtype == 1, stream);
+      break;
+    case 3:
+      launch_rows<3>(a, store, p.dtype == 1, stream);
+      break;
+    default:
+      launch_rows<4>(a, store, p.dtype == 1, stream);
+  }
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) {
+    set_error("%s: launch failed: %s", what, hipGetErrorString(e));
+    return TILEMIX_E_LAUNCH;
+  }
+  return TILEMIX_OK;
+}
+
+}  // namespace
+
+int launch_kv4_store(const tilemix_kv4_rows_params& p, hipStream_t stream) {
+  return run_rows("tilemix_kv4_store", p, true, stream);
+}
+int launch_kv4_load(const tilemix_kv4_rows_params& p, hipStream_t stream) {
+  return run_rows("tilemix_kv4_load", p, false, stream);
+}
+
+}  // namespace tmx
