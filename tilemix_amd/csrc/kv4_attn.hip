@@ -151,15 +151,13 @@ __device__ __forceinline__ int page_of(const Kv4Args& a, const int32_t* table, i
   return id < a.pages ? id : -1;
 }
 
+// The lane's part of a tile.  Keys without a page read rows of page 0 (there is one): no branch
+// around the loads; they count for nothing, whatever they hold.
 template <int NG>
 __device__ __forceinline__ void load_tile(Kv4Tile<NG>& x, const Kv4Args& a, int h, int key, int page) {
   const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
-  if (page < 0) {
-    x = Kv4Tile<NG>{};
-    return;
-  }
   const int column = fast_div(key, a.by_page);
-  const int64_t row = ((int64_t)page * a.hk + h) * a.by_page.d + (key - column * a.by_page.d) + (i & 3);
+  const int64_t row = ((int64_t)max(page, 0) * a.hk + h) * a.by_page.d + (key - column * a.by_page.d) + (i & 3);
   const uint32_t* const kc = a.kc + row * (4 * NG) + NG * g;
   const uint32_t* const vc = a.vc + row * (4 * NG) + NG * g;
   const uint32_t* const kp = a.kp + row * NG;
@@ -200,7 +198,8 @@ __global__ void __launch_bounds__(kWaves * 64, 2) kv4_attn_kernel(const Kv4Args 
     const int row = row0 + 16 * rt + i, token = fast_div(row, a.by_group), head = row - token * a.group;
     const bool there = row < it.rows;
     limit[rt] = a.causal ? it.limit0 + token : it.len;
-    scale[rt] = a.scale;
+    // A negative scale is the queries' sign; none is a product that leaves the maximum at zero.
+    scale[rt] = fmaxf(fabsf(a.scale), 1e-37f);
     const int64_t at = (it.start + token) * a.sq_t + (it.h * a.group + head) * a.sq_h;
     f32x8 x[NG];
     float top = 0.0f;
@@ -244,8 +243,8 @@ __global__ void __launch_bounds__(kWaves * 64, 2) kv4_attn_kernel(const Kv4Args 
     for (int s = 0; s < NG; ++s)
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        qf[rt][s][2 * j] = (f16)x[s][j];
-        qf[rt][s][2 * j + 1] = (f16)x[s][j + 4];
+        qf[rt][s][2 * j] = (f16)(a.scale < 0.0f ? -x[s][j] : x[s][j]);
+        qf[rt][s][2 * j + 1] = (f16)(a.scale < 0.0f ? -x[s][j + 4] : x[s][j + 4]);
       }
   }
 
@@ -276,9 +275,9 @@ __global__ void __launch_bounds__(kWaves * 64, 2) kv4_attn_kernel(const Kv4Args 
   for (; tile < last; tile += kWaves) {
     const int key0 = tile * kTile;
     const uint64_t pages = __ballot(page >= 0);
-    // keys behind the last one that any row sees may hold anything: they become zeros
+    // keys without a page and behind the last one that any row sees may hold anything: they become zeros
     {
-      const bool gone = key0 + key_i + 4 * g + (i & 3) >= it.kmax;
+      const bool gone = page < 0 || key0 + key_i + 4 * g + (i & 3) >= it.kmax;
 #pragma unroll
       for (int j = 0; j < NG; ++j) x.vp[j] = gone ? 0u : x.vp[j];
     }
@@ -345,9 +344,6 @@ __global__ void __launch_bounds__(kWaves * 64, 2) kv4_attn_kernel(const Kv4Args 
     const bool mine_there = (pages >> (4 * g)) & 1;
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-      // the scale may be negative: it comes before the maximum
-#pragma unroll
-      for (int t = 0; t < 4; ++t) acc[rt][t] *= scale[rt];
       if (masked) {
 #pragma unroll
         for (int t = 0; t < 4; ++t)
@@ -360,7 +356,7 @@ __global__ void __launch_bounds__(kWaves * 64, 2) kv4_attn_kernel(const Kv4Args 
       for (int t = 0; t < 4; ++t)
 #pragma unroll
         for (int e = 0; e < 4; ++e) hi = fmaxf(hi, acc[rt][t][e]);
-      hi = lanes16_max(hi);
+      hi = lanes16_max(hi) * scale[rt];
       if (__any(hi > top[rt] + kKv4Slack)) {
         const float up = fmaxf(hi, top[rt]), down = __builtin_amdgcn_exp2f(top[rt] - up);
         top[rt] = up;
@@ -372,7 +368,7 @@ __global__ void __launch_bounds__(kWaves * 64, 2) kv4_attn_kernel(const Kv4Args 
       for (int t = 0; t < 4; ++t)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          acc[rt][t][e] = __builtin_amdgcn_exp2f(acc[rt][t][e] - top[rt]);
+          acc[rt][t][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[rt][t][e], scale[rt], -top[rt]));
           sum[rt] += acc[rt][t][e];
         }
 #pragma unroll
@@ -503,30 +499,51 @@ __global__ void __launch_bounds__(kWaves * 64, 2) kv4_attn_kernel(const Kv4Args 
   }
 }
 
-// Adds up the splits of a row: one thread per four channels.
+// Adds up the splits of a row.  One thread takes four channels of every `lanes`-th split and keeps
+// its own running maximum; the `lanes` threads of a row's channels meet in LDS.
 template <int NG>
-__global__ void __launch_bounds__(256) kv4_join_kernel(const Kv4Args a, int block_rows) {
-  constexpr int kLanes = 8 * NG, kRows = 256 / kLanes;
-  const int r = threadIdx.x / kLanes, c = 4 * (threadIdx.x - r * kLanes);
-  const int groups = (block_rows + kRows - 1) / kRows, rb = blockIdx.x / groups;
-  const int in_block = (blockIdx.x - rb * groups) * kRows + r;
+__global__ void __launch_bounds__(256) kv4_join_kernel(const Kv4Args a, int block_rows, int lanes, int rows) {
+  constexpr int kC = 8 * NG;
+  __shared__ f32x4 lds_o[256];
+  __shared__ float2 lds_ml[256];
+  const int unit = threadIdx.x / kC, c = 4 * (threadIdx.x - unit * kC), r = unit / lanes, lane = unit - r * lanes;
+  const int groups = (block_rows + rows - 1) / rows, rb = blockIdx.x / groups;
+  const int in_block = (blockIdx.x - rb * groups) * rows + r;
   const Kv4Item it = kv4_item(a, blockIdx.z, blockIdx.y, rb, block_rows);
   const int row = rb * block_rows + in_block;
-  if (r >= kRows || in_block >= block_rows || row >= it.rows || c >= a.d) return;
-  const int tiles = it.kmax <= 0 ? 0 : (it.kmax + kTile - 1) / kTile;
-  const int parts = max(1, (tiles + a.split_tiles - 1) / a.split_tiles);
-  const int64_t first =
-      (int64_t)((it.b * a.hk + it.h) * a.row_blocks + rb) * a.splits * block_rows + in_block;
-  float top = kNoKey;
-  for (int s = 0; s < parts; ++s) top = fmaxf(top, a.part_ml[first + (int64_t)s * block_rows].x);
+  const bool there = r < rows && in_block < block_rows && row < it.rows;
   f32x4 o = {};
-  float sum = 0.0f;
-  for (int s = 0; s < parts; ++s) {
-    const int64_t at = first + (int64_t)s * block_rows;
-    const float2 ml = a.part_ml[at];
-    const float down = __builtin_amdgcn_exp2f(ml.x - top);
-    sum += ml.y * down;
-    o += *reinterpret_cast<const f32x4*>(a.part + at * (32 * NG) + c) * down;
+  float2 ml = make_float2(kNoKey, 0.0f);
+  if (there) {
+    const int tiles = it.kmax <= 0 ? 0 : (it.kmax + kTile - 1) / kTile;
+    const int parts = max(1, (tiles + a.split_tiles - 1) / a.split_tiles);
+    const int64_t first =
+        (int64_t)((it.b * a.hk + it.h) * a.row_blocks + rb) * a.splits * block_rows + in_block;
+#pragma unroll 4
+    for (int s = lane; s < parts; s += lanes) {
+      const int64_t at = first + (int64_t)s * block_rows;
+      const float2 part = a.part_ml[at];
+      const f32x4 x = *reinterpret_cast<const f32x4*>(a.part + at * (32 * NG) + c);
+      const float up = fmaxf(ml.x, part.x);
+      const float mine = __builtin_amdgcn_exp2f(ml.x - up), its = __builtin_amdgcn_exp2f(part.x - up);
+      ml = make_float2(up, ml.y * mine + part.y * its);
+      o = o * mine + x * its;
+    }
+  }
+  lds_o[threadIdx.x] = o;
+  lds_ml[threadIdx.x] = ml;
+  __syncthreads();
+  if (!there || lane != 0 || c >= a.d) return;
+  float top = ml.x;
+  for (int i = 1; i < lanes; ++i) top = fmaxf(top, lds_ml[threadIdx.x + i * kC].x);
+  const float mine = __builtin_amdgcn_exp2f(ml.x - top);
+  o *= mine;
+  float sum = ml.y * mine;
+  for (int i = 1; i < lanes; ++i) {
+    const float2 part = lds_ml[threadIdx.x + i * kC];
+    const float its = __builtin_amdgcn_exp2f(part.x - top);
+    sum += part.y * its;
+    o += lds_o[threadIdx.x + i * kC] * its;
   }
   o *= sum == 0.0f ? 0.0f : 1.0f / sum;
   const int token = fast_div(row, a.by_group), head = row - token * a.group;
@@ -583,9 +600,13 @@ void launch_kv4(const Kv4Args& a, int batch, hipStream_t stream) {
   hipLaunchKernelGGL((kv4_attn_kernel<NG, RT>), dim3((unsigned)(a.row_blocks * a.splits), a.hk, batch),
                      dim3(kWaves * 64), lds, stream, a);
   if (a.splits > 1) {
-    constexpr int rows = 256 / (8 * NG);
+    // about four splits a thread
+    constexpr int units = 256 / (8 * NG);
+    int lanes = 1;
+    while (lanes * 2 <= units && lanes * 4 < a.splits) lanes *= 2;
+    const int rows = units / lanes;
     hipLaunchKernelGGL((kv4_join_kernel<NG>), dim3((unsigned)(a.row_blocks * ((16 * RT + rows - 1) / rows)), a.hk, batch),
-                       dim3(256), 0, stream, a, 16 * RT);
+                       dim3(256), 0, stream, a, 16 * RT, lanes, rows);
   }
 }
 

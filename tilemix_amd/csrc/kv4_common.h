@@ -8,6 +8,13 @@ namespace tmx {
 constexpr int kKv4Group = 32;          // channels that share a scale and a minimum
 constexpr float kKv4Limit = 65408.0f;  // values are clamped here: 15 s + m < 65520 then rounds to a finite fp16
 
+// (x & mask) | bits in one instruction (the compiler takes two, each with a literal: VOP3 has none).
+__device__ __forceinline__ f16x2 kv4_and_or(uint32_t x, uint32_t mask, uint32_t bits) {
+  uint32_t r;
+  asm("v_and_or_b32 %0, %1, %2, %3" : "=v"(r) : "v"(x), "s"(mask), "v"(bits));
+  return __builtin_bit_cast(f16x2, r);
+}
+
 // The eight codes of a word as four pairs of fp16 whole numbers, channels (0, 4), (1, 5), (2, 6),
 // (3, 7).  A code in the low four bits of fp16 1024 (one unit in the last place) reads 1024 + n, in the
 // next four of 64 it reads 64 + n; the subtraction is exact.
@@ -15,10 +22,10 @@ __device__ __forceinline__ void kv4_codes(uint32_t w, f16x2 (&n)[4]) {
   const uint32_t lo = 0x000f000fu, hi = 0x00f000f0u, k1024 = 0x64006400u, k64 = 0x54005400u;
   const f16x2 m1024 = {(f16)-1024.0f, (f16)-1024.0f}, m64 = {(f16)-64.0f, (f16)-64.0f};
   const uint32_t u = w >> 8;
-  n[0] = __builtin_bit_cast(f16x2, (w & lo) | k1024) + m1024;
-  n[1] = __builtin_bit_cast(f16x2, (w & hi) | k64) + m64;
-  n[2] = __builtin_bit_cast(f16x2, (u & lo) | k1024) + m1024;
-  n[3] = __builtin_bit_cast(f16x2, (u & hi) | k64) + m64;
+  n[0] = kv4_and_or(w, lo, k1024) + m1024;
+  n[1] = kv4_and_or(w, hi, k64) + m64;
+  n[2] = kv4_and_or(u, lo, k1024) + m1024;
+  n[3] = kv4_and_or(u, hi, k64) + m64;
 }
 
 __device__ __forceinline__ f16x2 kv4_fma(f16x2 n, f16x2 s, f16x2 m) { return __builtin_elementwise_fma(n, s, m); }
