@@ -261,7 +261,7 @@ int tilemix_silu_mul_f16(const void* gate, const void* up, void* out, int64_t n,
 
 /*
  * The paged 4-bit KV cache.  A pool holds `pages` pages of `page_size` token rows
- * (a multiple of 16) for each of `heads` KV heads.  A row's head_dim values (at most
+ * (a multiple of 16) for each of `heads` KV heads, fewer than 2^31 in all.  A row's head_dim values (at most
  * 128) are split into groups of 32 channels; NG = ceil(head_dim / 32).  A group has a
  * scale s and a minimum m in fp16 and a 4-bit code n a channel:
  *   x' = min(max(x, -65408), 65408)     (so that no value below overflows fp16)

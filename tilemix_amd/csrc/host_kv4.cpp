@@ -96,6 +96,8 @@ Pool pool(PyObject* const* a) {
                     ", got ", codes.sizes());
   TORCH_CHECK_VALUE(codes.size(2) >= 16 && codes.size(2) % 16 == 0 && codes.size(2) <= (1 << 24),
                     "page_size must be a positive multiple of 16, got ", codes.size(2));
+  TORCH_CHECK_VALUE(codes.size(0) * codes.size(1) <= INT32_MAX / codes.size(2), "a cache has fewer than 2^31 rows, got ",
+                    codes.sizes());
   p.pages = static_cast<int>(codes.size(0));
   p.heads = static_cast<int>(codes.size(1));
   p.page_size = static_cast<int>(codes.size(2));

@@ -100,27 +100,29 @@ __device__ __forceinline__ uint32_t lanes16_or(uint32_t x) {
 
 // ---- lane layouts ---------------------------------------------------------------
 // Lane l = 16 g + i of a wave.  Matrix operands of 16x16x32: A holds row i, B column i, both the
-// k-slots 8 g .. 8 g + 7; the result holds column i and rows 4 g .. 4 g + 3.
-//  * QK: A = K.  Of a tile's four groups of 16 result rows, t = 0 .. 3, row i is key
-//    16 (i / 4) + 4 t + i % 4: result rows 4 g + e are then keys 16 g + 4 t + e, so a lane ends up with
-//    the 16 consecutive keys 16 g .. 16 g + 15 of query row i.  The slots of step s are the
-//    channels of word NG g + s of a row (word: eight channels), in the pairs of kv4_codes: a lane
-//    reads NG consecutive words of a key, whose group is theirs alone (NG = 3: one of two).
+// k-slots 8 g .. 8 g + 7; the result holds column i and rows 4 g .. 4 g + 3.  A tile is four blocks
+// t = 0 .. 3 of 16 keys; a block lies in one page, so that its rows have one scalar base.
+//  * QK: A = K, row i = key 16 t + i.  The slots of step s are the channels of word NG g + s of a row
+//    (word: eight channels), in the pairs of kv4_codes: a lane reads NG consecutive words of a
+//    key, whose group is theirs alone (NG = 3: one of two).  Result: keys 16 t + 4 g + e of query row i.
 //  * PV: A = V^T through ds_read_b64_tr_b4, which transposes a 16 x 16 block of codes in each 16 lanes:
-//    lane i gets channel i of the 16 rows that the lanes point at, here keys 16 g .. 16 g + 15.
-//    Word w of it are keys 16 g + 8 w .. + 7, in the pairs (0, 4), (1, 5) ..: the pairs
-//    (S[2 w][e], S[2 w + 1][e]) of the lane's own results, so P stays in registers.
+//    lane i gets channel i of the 16 rows that the lanes point at, in their order.  Lane i of
+//    group g points at key 16 (i / 4) + 4 g + i % 4: code 4 t + e of the result is the key that the lane
+//    holds as result e of block t, so P stays in registers.  Word w of it are blocks 2 w
+//    and 2 w + 1, in the pairs (0, 4), (1, 5) .. of kv4_codes: e of the one with e of the other.
 template <int NG>
 struct Kv4Tile {
-  static constexpr int kW = NG;              // words of a lane's part of a K or V row
-  static constexpr int kNP = NG == 3 ? 2 : 1;  // groups that these words can lie in
-  static constexpr int kStride = 16 * NG + 8;  // bytes of a V row in LDS: odd in 8-byte units, no bank conflicts
-  uint32_t k[4][kW], v[4][kW], kp[4][kNP], vp[NG];
+  static constexpr int kNP = NG == 3 ? 2 : 1;  // groups that a lane's words of a K row can lie in
+  uint32_t k[4][NG], kp[4][kNP], vp[4];
 };
 
-// LDS of one wave: V codes, then the scales and minima [NG][64] each in the key order of the pairs.
+// LDS of one wave: two tiles of V codes, then the scales and minima [NG][64] of a tile in the pairs' order.
+// A block of V is [chunk of 16 bytes][key] as the copies write it (lane l: byte 16 l); the blocks
+// lie 64 bytes more than 1 KB apart, which leaves the transposed reads two lanes to a bank, their least
+// while they read one half of each chunk.
+constexpr int kBlockLds = 1024 + 64;
 template <int NG>
-constexpr int kWaveLds = 64 * Kv4Tile<NG>::kStride + NG * 64 * 4;
+constexpr int kWaveLds = 2 * 4 * kBlockLds + NG * 64 * 4;
 
 template <int NG, int RT>
 constexpr int kv4_lds_bytes() {
@@ -144,43 +146,117 @@ __device__ __forceinline__ void load_words(uint32_t (&to)[N], const uint32_t* fr
   }
 }
 
-// The page of the lane's 16 keys 16 (i / 4) .. + 15 of a tile: -1 where there is none.
-__device__ __forceinline__ int page_of(const Kv4Args& a, const int32_t* table, int key, int kmax) {
-  if (key >= kmax) return -1;
-  const int id = table[fast_div(key, a.by_page)];
-  return id < a.pages ? id : -1;
+// 16 bytes a lane from base + offset to LDS: lane l writes lds + 16 l.  As async_load16_asm
+// (attn_common.h), from a scalar address; the same five wait states.
+__device__ __forceinline__ void copy16(const uint32_t* base, uint32_t offset, uint32_t lds) {
+  asm volatile(
+      "s_nop 4\n\t"
+      "global_load_lds_dwordx4 %0, %1"
+      :
+      : "v"(offset), "s"(base), "{m0}"(lds)
+      : "memory");
 }
 
-// The lane's part of a tile.  Keys without a page read rows of page 0 (there is one): no branch
-// around the loads; they count for nothing, whatever they hold.
+// The keys of one wave: tiles first + wave, + kWaves, ..  Tile n of them has its blocks' rows of the pool
+// in the lanes 4 (n % 16) .. + 3 of `rows` (-1: no page, or behind `end`), from one load of the block table for
+// every 16 tiles, made 16 tiles ahead.
+struct Kv4Walk {
+  const int32_t* table;
+  int key0, end;  // first key of the wave; no block at or behind `end`
+  int rows, ids;
+
+  __device__ __forceinline__ int key(int n) const {
+    const int lane = threadIdx.x & 63;
+    return key0 + (n + (lane >> 2)) * (kWaves * kTile) + 16 * (lane & 3);
+  }
+  __device__ __forceinline__ int fetch(const Kv4Args& a, int n) const {
+    const int k = key(n);
+    return k < end ? table[fast_div(k, a.by_page)] : -1;
+  }
+  __device__ __forceinline__ void use(const Kv4Args& a, int h, int n) {
+    const int k = key(n), column = fast_div(k, a.by_page);
+    rows = ids >= 0 && ids < a.pages ? (ids * a.hk + h) * a.by_page.d + (k - column * a.by_page.d) : -1;
+  }
+};
+
+// Starts the loads of tile n (V codes into LDS); there: which of its blocks have a page.  A block without
+// one reads rows of page 0 (there is one): no branch around the loads; they count for nothing, whatever
+// they hold.
 template <int NG>
-__device__ __forceinline__ void load_tile(Kv4Tile<NG>& x, const Kv4Args& a, int h, int key, int page) {
-  const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
-  const int column = fast_div(key, a.by_page);
-  const int64_t row = ((int64_t)max(page, 0) * a.hk + h) * a.by_page.d + (key - column * a.by_page.d) + (i & 3);
-  const uint32_t* const kc = a.kc + row * (4 * NG) + NG * g;
-  const uint32_t* const vc = a.vc + row * (4 * NG) + NG * g;
-  const uint32_t* const kp = a.kp + row * NG;
+__device__ __forceinline__ uint32_t load_tile(Kv4Tile<NG>& x, const Kv4Args& a, const Kv4Walk& walk, int n,
+                                              uint32_t lds_v) {
+  const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4, gc = g < NG ? g : NG - 1;
+  const uint32_t words_at = i * (4 * NG) + NG * g, chunk_at = 16 * (i * NG + gc), group_at = i * NG + gc;
+  uint32_t there = 0;
+  const uint32_t* base[4];
+  int64_t row[4];
 #pragma unroll
   for (int t = 0; t < 4; ++t) {
-    load_words(x.k[t], kc + t * (16 * NG));
-#pragma unroll
-    for (int j = 0; j < Kv4Tile<NG>::kNP; ++j) {
-      const int group = NG == 4 ? g : j == 0 ? NG * g / 4 : (NG * g + NG - 1) / 4;
-      x.kp[t][j] = kp[t * (4 * NG) + group];
-    }
+    const int r = __builtin_amdgcn_readlane(walk.rows, 4 * (n & 15) + t);
+    there |= r >= 0 ? 1u << t : 0u;
+    row[t] = r >= 0 ? r : 0;
+    base[t] = a.kc + row[t] * (4 * NG);
   }
 #pragma unroll
-  for (int t = 0; t < 4; ++t) load_words(x.v[t], vc + t * (16 * NG));
-  load_words(x.vp, a.vp + (row + 4 * g) * NG);  // of key 16 (i / 4) + 4 g + i % 4
+  for (int t = 0; t < 4; ++t) copy16(a.vc + row[t] * (4 * NG), chunk_at, lds_v + t * kBlockLds);
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+    load_words(x.k[t], base[t] + words_at);
+#pragma unroll
+    for (int j = 0; j < Kv4Tile<NG>::kNP; ++j) {
+      const uint32_t group = NG == 4 ? g : j == 0 ? NG * g / 4 : (NG * g + NG - 1) / 4;
+      x.kp[t][j] = (a.kp + row[t] * NG)[i * NG + group];
+    }
+    x.vp[t] = (a.vp + row[t] * NG)[group_at];
+  }
+  return there;
+}
+
+// Elements c .. c + n - 1 (n <= 8) of a query row, zeros behind them.
+__device__ __forceinline__ f32x8 load_query(const uint16_t* row, int c, int n, bool vec, bool bf) {
+  u32x4 w;
+  if (vec && n == 8) {
+    w = *reinterpret_cast<const u32x4*>(row + c);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t lo = row[2 * e < n ? c + 2 * e : 0], hi = row[2 * e + 1 < n ? c + 2 * e + 1 : 0];
+      w[e] = (2 * e < n ? lo : 0u) | (2 * e + 1 < n ? hi << 16 : 0u);
+    }
+  }
+  f32x8 x;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const uint32_t pair = w[e];  // (a bit cast of a vector's element would take the first one)
+    const f16x2 h = __builtin_bit_cast(f16x2, pair);
+    x[2 * e] = bf ? __uint_as_float(pair << 16) : (float)h[0];
+    x[2 * e + 1] = bf ? __uint_as_float(pair & 0xffff0000u) : (float)h[1];
+  }
+  return x;
+}
+
+// Rounds four channels to the output's type and writes those below d.
+__device__ __forceinline__ void store_out(void* out, int64_t at, const f32x4& r, int left, bool vec, bool bf) {
+  uint16_t* const to = static_cast<uint16_t*>(out) + at;
+  const uint2 v = bf ? __builtin_bit_cast(uint2, __builtin_convertvector(r, bf16x4))
+                     : __builtin_bit_cast(uint2, __builtin_convertvector(r, f16x4));
+  if (vec && left >= 4) {
+    *reinterpret_cast<uint2*>(to) = v;
+  } else {
+    if (left > 0) to[0] = (uint16_t)v.x;
+    if (left > 1) to[1] = (uint16_t)(v.x >> 16);
+    if (left > 2) to[2] = (uint16_t)v.y;
+    if (left > 3) to[3] = (uint16_t)(v.y >> 16);
+  }
 }
 
 template <int NG, int RT>
-__global__ void __launch_bounds__(kWaves * 64, 2) kv4_attn_kernel(const Kv4Args a) {
+__global__ void __launch_bounds__(kWaves * 64, RT == 1 ? 3 : 2) kv4_attn_kernel(const Kv4Args a) {
   using Tile = Kv4Tile<NG>;
   constexpr int kCT = 2 * NG;  // tiles of 16 channels
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, g = lane >> 4;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15,
+            g = lane >> 4;
   const int rb = fast_div(blockIdx.x, a.by_splits), split = blockIdx.x - rb * a.splits;
   const Kv4Item it = kv4_item(a, blockIdx.z, blockIdx.y, rb, 16 * RT);
   const int row0 = rb * 16 * RT;
@@ -188,6 +264,13 @@ __global__ void __launch_bounds__(kWaves * 64, 2) kv4_attn_kernel(const Kv4Args 
   const int tiles = it.kmax <= 0 ? 0 : (it.kmax + kTile - 1) / kTile;
   const int first = split * a.split_tiles, last = min(tiles, first + a.split_tiles);
   if (first >= last && split > 0) return;
+
+  // ---- the first keys' places are on their way while the queries come ----
+  Kv4Walk walk;
+  walk.table = a.table + it.b * a.s_table;
+  walk.key0 = (first + wave) * kTile;
+  walk.end = min(it.kmax, last * kTile);
+  walk.ids = walk.fetch(a, 0);
 
   // ---- queries: B operand of QK, rows 16 rt + i ----
   f16x8 qf[RT][NG];
@@ -200,32 +283,16 @@ __global__ void __launch_bounds__(kWaves * 64, 2) kv4_attn_kernel(const Kv4Args 
     limit[rt] = a.causal ? it.limit0 + token : it.len;
     // A negative scale is the queries' sign; none is a product that leaves the maximum at zero.
     scale[rt] = fmaxf(fabsf(a.scale), 1e-37f);
-    const int64_t at = (it.start + token) * a.sq_t + (it.h * a.group + head) * a.sq_h;
+    // a row that is not there reads the block's first one and becomes zeros
+    const uint16_t* const from =
+        static_cast<const uint16_t*>(a.q) + (it.start + (there ? token : fast_div(row0, a.by_group))) * a.sq_t +
+        (it.h * a.group + (there ? head : row0 - fast_div(row0, a.by_group) * a.group)) * a.sq_h;
     f32x8 x[NG];
     float top = 0.0f;
 #pragma unroll
     for (int s = 0; s < NG; ++s) {
       const int c = 8 * (NG * g + s), n = there ? min(8, a.d - c) : 0;
-      x[s] = f32x8{};
-      if (a.bf) {
-        const bf16* const from = static_cast<const bf16*>(a.q) + at + c;
-        if (a.q_vec && n == 8) {
-          x[s] = __builtin_convertvector(*reinterpret_cast<const bf16x8*>(from), f32x8);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if (e < n) x[s][e] = (float)from[e];
-        }
-      } else {
-        const f16* const from = static_cast<const f16*>(a.q) + at + c;
-        if (a.q_vec && n == 8) {
-          x[s] = __builtin_convertvector(*reinterpret_cast<const f16x8*>(from), f32x8);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if (e < n) x[s][e] = (float)from[e];
-        }
-      }
+      x[s] = load_query(from, c, n, a.q_vec, a.bf);
 #pragma unroll
       for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[s][e]));
     }
@@ -259,55 +326,51 @@ __global__ void __launch_bounds__(kWaves * 64, 2) kv4_attn_kernel(const Kv4Args 
   }
 
   unsigned char* const lds_v = smem + wave * kWaveLds<NG>;
-  f16* const lds_s = reinterpret_cast<f16*>(lds_v + 64 * Tile::kStride);
+  f16* const lds_s = reinterpret_cast<f16*>(lds_v + 2 * 4 * kBlockLds);
   f16* const lds_m = lds_s + NG * 64;
-  const int32_t* const table = a.table + it.b * a.s_table;
+  const uint32_t v_addr = lds_addr(lds_v);
   const int all_see = it.limit0 + (a.causal ? fast_div(row0, a.by_group) : 0);  // keys that every row sees
-  const int key_i = 16 * (i >> 2);  // first of the lane's 16 keys of a tile
-  // position of key 4 g + i % 4 of 16 in the pairs' order (0, 4), (1, 5), (2, 6), (3, 7), (8, 12) ..
-  const int p_at = key_i + 8 * (g >> 1) + 2 * (i & 3) + (g & 1);
+  // V rows that the lane points at in a transposed read, in LDS
+  const int v_at = (i >> 2) * kBlockLds + (4 * g + (i & 3)) * 16;
+  const int p_at = 16 * (i >> 2) + 2 * (i & 3);  // of key i of a block in the pairs' order, see below
 
   Tile x;
-  int tile = first + wave;
-  int page = page_of(a, table, tile * kTile + key_i, min(it.kmax, last * kTile));
-  int next = page_of(a, table, (tile + kWaves) * kTile + key_i, min(it.kmax, last * kTile));
-  load_tile(x, a, it.h, tile * kTile + key_i, page);
-  for (; tile < last; tile += kWaves) {
+  walk.use(a, it.h, 0);
+  walk.ids = walk.fetch(a, 16);
+  uint32_t there = load_tile(x, a, walk, 0, v_addr);
+  int n = 0;
+  for (int tile = first + wave; tile < last; tile += kWaves, ++n) {
     const int key0 = tile * kTile;
-    const uint64_t pages = __ballot(page >= 0);
-    // keys without a page and behind the last one that any row sees may hold anything: they become zeros
-    {
-      const bool gone = page < 0 || key0 + key_i + 4 * g + (i & 3) >= it.kmax;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the copies of V; the other loads are as old
+    const bool masked = key0 + kTile > all_see || there != 15u;
+    if (masked) {
+      // rows without a page and behind the last key that any row sees may hold anything: zeros
 #pragma unroll
-      for (int j = 0; j < NG; ++j) x.vp[j] = gone ? 0u : x.vp[j];
+      for (int t = 0; t < 4; ++t)
+        if (!((there >> t) & 1) || key0 + 16 * t + i >= it.kmax) x.vp[t] = 0;
     }
-    uint32_t broken = 0;  // groups of the lane's key whose values are not finite: zeros here, see below
+    // groups whose values are not finite: zeros here, see below
+    uint64_t broken[4];
+    bool any_broken = false;
 #pragma unroll
-    for (int j = 0; j < NG; ++j)
-      if (kv4_not_finite(x.vp[j])) {
-        broken |= 1u << j;
-        x.vp[j] = 0;
-      }
-    // ---- V codes and parameters to LDS ----
+    for (int t = 0; t < 4; ++t) any_broken |= kv4_not_finite(x.vp[t]);
+    any_broken = __any(any_broken);
+    if (any_broken) {
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      uint32_t* const to =
-          reinterpret_cast<uint32_t*>(lds_v + (key_i + 4 * t + (i & 3)) * Tile::kStride) + Tile::kW * g;
-      if constexpr (NG == 4) {
-        *reinterpret_cast<uint2*>(to) = make_uint2(x.v[t][0], x.v[t][1]);
-        *reinterpret_cast<uint2*>(to + 2) = make_uint2(x.v[t][2], x.v[t][3]);
-      } else if constexpr (NG == 2) {
-        *reinterpret_cast<uint2*>(to) = make_uint2(x.v[t][0], x.v[t][1]);
-      } else {
-#pragma unroll
-        for (int s = 0; s < NG; ++s) to[s] = x.v[t][s];
+      for (int t = 0; t < 4; ++t) {
+        const bool bad = kv4_not_finite(x.vp[t]);
+        broken[t] = __ballot(bad);
+        if (bad) x.vp[t] = 0;
       }
     }
+    // ---- V's parameters to LDS: pairs of the same key of blocks 2 w and 2 w + 1 ----
+    if (NG == 4 || g < NG) {
 #pragma unroll
-    for (int j = 0; j < NG; ++j) {
-      const f16x2 sm = __builtin_bit_cast(f16x2, x.vp[j]);
-      lds_s[j * 64 + p_at] = sm[0];
-      lds_m[j * 64 + p_at] = sm[1];
+      for (int w = 0; w < 2; ++w) {
+        const uint32_t p0 = x.vp[2 * w], p1 = x.vp[2 * w + 1];
+        *reinterpret_cast<uint32_t*>(lds_s + g * 64 + p_at + 8 * w) = __builtin_amdgcn_perm(p1, p0, 0x05040100u);
+        *reinterpret_cast<uint32_t*>(lds_m + g * 64 + p_at + 8 * w) = __builtin_amdgcn_perm(p1, p0, 0x07060302u);
+      }
     }
     // ---- S^T = K Q^T ----
     f32x4 acc[RT][4];
@@ -319,12 +382,12 @@ __global__ void __launch_bounds__(kWaves * 64, 2) kv4_attn_kernel(const Kv4Args 
       for (int s = 0; s < NG; ++s) {
         const uint32_t p = NG == 3 && (NG * g + s) / 4 != NG * g / 4 ? x.kp[t][Tile::kNP - 1] : x.kp[t][0];
         const f16x2 sm = __builtin_bit_cast(f16x2, p), sc = {sm[0], sm[0]}, mn = {sm[1], sm[1]};
-        f16x2 n[4];
-        kv4_codes(x.k[t][s], n);
+        f16x2 c[4];
+        kv4_codes(x.k[t][s], c);
         f16x8 kf;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const f16x2 v = kv4_fma(n[j], sc, mn);
+          const f16x2 v = kv4_fma(c[j], sc, mn);
           kf[2 * j] = v[0];
           kf[2 * j + 1] = v[1];
         }
@@ -333,15 +396,18 @@ __global__ void __launch_bounds__(kWaves * 64, 2) kv4_attn_kernel(const Kv4Args 
           acc[rt][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[rt][s], acc[rt][t], 0, 0, 0);
       }
     }
+    __builtin_amdgcn_sched_barrier(0);
     // ---- the next tile is on its way while this one goes on ----
-    page = next;
-    load_tile(x, a, it.h, key0 + kWaves * kTile + key_i, page);
-    next = page_of(a, table, key0 + 2 * kWaves * kTile + key_i, min(it.kmax, last * kTile));
+    const uint32_t here = there;
+    if (((n + 1) & 15) == 0) {
+      walk.use(a, it.h, n + 1);
+      walk.ids = walk.fetch(a, n + 17);
+    }
+    there = load_tile(x, a, walk, n + 1, v_addr + ((n + 1) & 1) * 4 * kBlockLds);
+    __builtin_amdgcn_sched_barrier(0);
     // ---- softmax ----
-    const bool masked = key0 + kTile > all_see || pages != ~0ull;
     f16x8 pf[RT][2];
-    const int mine = key0 + 16 * g;  // the lane's 16 keys
-    const bool mine_there = (pages >> (4 * g)) & 1;
+    const int mine = key0 + 4 * g;  // the lane's keys are mine + 16 t + e
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
       if (masked) {
@@ -349,7 +415,7 @@ __global__ void __launch_bounds__(kWaves * 64, 2) kv4_attn_kernel(const Kv4Args 
         for (int t = 0; t < 4; ++t)
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            if (!mine_there || mine + 4 * t + e >= limit[rt]) acc[rt][t][e] = -__builtin_inff();
+            if (!((here >> t) & 1) || mine + 16 * t + e >= limit[rt]) acc[rt][t][e] = -__builtin_inff();
       }
       float hi = -__builtin_inff();
 #pragma unroll
@@ -380,9 +446,11 @@ __global__ void __launch_bounds__(kWaves * 64, 2) kv4_attn_kernel(const Kv4Args 
         }
     }
     // ---- O^T += V^T P^T ----
-    const unsigned char* const v_at = lds_v + (16 * g + i) * Tile::kStride;
+    const unsigned char* const v_tile = lds_v + (n & 1) * 4 * kBlockLds + v_at;
 #pragma unroll
     for (int j = 0; j < NG; ++j) {
+      // (one group's parameters at a time: fetched all ahead they would take 64 registers)
+      __builtin_amdgcn_sched_barrier(0);
       f16x2 sc[8], mn[8];
 #pragma unroll
       for (int w = 0; w < 2; ++w) {
@@ -398,15 +466,15 @@ __global__ void __launch_bounds__(kWaves * 64, 2) kv4_attn_kernel(const Kv4Args 
       for (int c = 0; c < 2; ++c) {
         const int ct = 2 * j + c;
         const i32x2 words = __builtin_amdgcn_ds_read_tr4_b64_v2i32(
-            (__attribute__((address_space(3))) i32x2*)(v_at + 8 * ct));
+            (__attribute__((address_space(3))) i32x2*)(v_tile + 256 * j + 8 * c));
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
-          f16x2 n[4];
-          kv4_codes((uint32_t)words[w], n);
+          f16x2 code[4];
+          kv4_codes((uint32_t)words[w], code);
           f16x8 vf;
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const f16x2 v = kv4_fma(n[e], sc[4 * w + e], mn[4 * w + e]);
+            const f16x2 v = kv4_fma(code[e], sc[4 * w + e], mn[4 * w + e]);
             vf[2 * e] = v[0];
             vf[2 * e + 1] = v[1];
           }
@@ -418,23 +486,29 @@ __global__ void __launch_bounds__(kWaves * 64, 2) kv4_attn_kernel(const Kv4Args 
     }
     // Values that are not finite (a NaN was stored): the rows that see the key get a NaN in the
     // group's channels, the others must not (0 times NaN would be one).
-    if (__any(broken != 0)) {
-      uint32_t seen[RT] = {};
+    if (any_broken) {
+      int at = 4 * g;
+      asm volatile("" : "+v"(at));  // what follows stays in this rare block
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) {
+        uint32_t seen = 0;  // groups
 #pragma unroll
-        for (int k = 0; k < 16; ++k) {
-          // key 16 g + k is held by the lane 16 (k / 4) + 4 g + k % 4
-          const uint32_t bad = __shfl(broken, 16 * (k >> 2) + 4 * g + (k & 3), 64);
-          if (mine + k < limit[rt]) seen[rt] |= bad;
+        for (int t = 0; t < 4; ++t) {
+          const uint32_t keys = (1u << min(max(limit[rt] - (key0 + 16 * t + at), 0), 4)) - 1;
+#pragma unroll
+          for (int j = 0; j < NG; ++j) {
+            const uint32_t bits = (uint32_t)(j < 2 ? broken[t] : broken[t] >> 32) >> (16 * (j & 1) + at);
+            seen |= (bits & keys) != 0 ? 1u << j : 0u;
+          }
         }
-        seen[rt] = lanes16_or(seen[rt]);
+        seen = lanes16_or(seen);
 #pragma unroll
         for (int ct = 0; ct < kCT; ++ct)
-          if ((seen[rt] >> (ct >> 1)) & 1) o[rt][ct] = f32x4{} + __builtin_nanf("");
+          if ((seen >> (ct >> 1)) & 1) o[rt][ct] = f32x4{} + __builtin_nanf("");
       }
     }
   }
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no copy is left that could overwrite what follows
 
   // ---- the four waves' parts ----
   float2* const lds_ml = reinterpret_cast<float2*>(smem + kv4_lds_bytes<NG, RT>() - kWaves * RT * 16 * 8);
@@ -476,24 +550,8 @@ __global__ void __launch_bounds__(kWaves * 64, 2) kv4_attn_kernel(const Kv4Args 
           continue;
         }
         r *= norm;
-        const int64_t at = (it.start + token) * a.so_t + (it.h * a.group + head) * a.so_h + c;
-        if (a.bf) {
-          bf16* const to = static_cast<bf16*>(a.out) + at;
-          const bf16x4 v = __builtin_convertvector(r, bf16x4);
-          if (a.o_vec && c + 4 <= a.d) *reinterpret_cast<bf16x4*>(to) = v;
-          else
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (c + e < a.d) to[e] = v[e];
-        } else {
-          f16* const to = static_cast<f16*>(a.out) + at;
-          const f16x4 v = __builtin_convertvector(r, f16x4);
-          if (a.o_vec && c + 4 <= a.d) *reinterpret_cast<f16x4*>(to) = v;
-          else
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (c + e < a.d) to[e] = v[e];
-        }
+        store_out(a.out, (it.start + token) * a.so_t + (it.h * a.group + head) * a.so_h + c, r, a.d - c, a.o_vec,
+                  a.bf);
       }
     }
   }
@@ -547,13 +605,7 @@ __global__ void __launch_bounds__(256) kv4_join_kernel(const Kv4Args a, int bloc
   }
   o *= sum == 0.0f ? 0.0f : 1.0f / sum;
   const int token = fast_div(row, a.by_group), head = row - token * a.group;
-  const int64_t at = (it.start + token) * a.so_t + (it.h * a.group + head) * a.so_h + c;
-#pragma unroll
-  for (int e = 0; e < 4; ++e)
-    if (c + e < a.d) {
-      if (a.bf) static_cast<bf16*>(a.out)[at + e] = (bf16)o[e];
-      else static_cast<f16*>(a.out)[at + e] = (f16)o[e];
-    }
+  store_out(a.out, (it.start + token) * a.so_t + (it.h * a.group + head) * a.so_h + c, o, a.d - c, a.o_vec, a.bf);
 }
 
 struct Plan {

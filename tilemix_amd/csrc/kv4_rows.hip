@@ -16,7 +16,7 @@ bool kv4_pool_ok(const char* what, const void* kc, const void* kp, const void* v
     return false;
   }
   if (pages <= 0 || page_size <= 0 || page_size % 16 != 0 || heads <= 0 || heads > 65535 || head_dim <= 0 ||
-      head_dim > 128 || (dtype != 0 && dtype != 1)) {
+      head_dim > 128 || (dtype != 0 && dtype != 1) || (int64_t)pages * heads > INT32_MAX / page_size) {
     set_error("%s: invalid cache (pages %d, page_size %d, heads %d, head_dim %d, dtype %d)", what, pages, page_size,
               heads, head_dim, dtype);
     return false;
