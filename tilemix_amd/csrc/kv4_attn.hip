@@ -250,32 +250,11 @@ __device__ __forceinline__ void store_out(void* out, int64_t at, const f32x4& r,
   }
 }
 
+// The queries of rows row0 + 16 rt + i as B operand of QK, the factor of their products and the keys they see.
 template <int NG, int RT>
-__global__ void __launch_bounds__(kWaves * 64, RT == 1 ? 3 : 2) kv4_attn_kernel(const Kv4Args a) {
-  using Tile = Kv4Tile<NG>;
-  constexpr int kCT = 2 * NG;  // tiles of 16 channels
-  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15,
-            g = lane >> 4;
-  const int rb = fast_div(blockIdx.x, a.by_splits), split = blockIdx.x - rb * a.splits;
-  const Kv4Item it = kv4_item(a, blockIdx.z, blockIdx.y, rb, 16 * RT);
-  const int row0 = rb * 16 * RT;
-  if (row0 >= it.rows) return;
-  const int tiles = it.kmax <= 0 ? 0 : (it.kmax + kTile - 1) / kTile;
-  const int first = split * a.split_tiles, last = min(tiles, first + a.split_tiles);
-  if (first >= last && split > 0) return;
-
-  // ---- the first keys' places are on their way while the queries come ----
-  Kv4Walk walk;
-  walk.table = a.table + it.b * a.s_table;
-  walk.key0 = (first + wave) * kTile;
-  walk.end = min(it.kmax, last * kTile);
-  walk.ids = walk.fetch(a, 0);
-
-  // ---- queries: B operand of QK, rows 16 rt + i ----
-  f16x8 qf[RT][NG];
-  float scale[RT];
-  int limit[RT];
+__device__ __forceinline__ void load_queries(const Kv4Args& a, const Kv4Item& it, int row0, f16x8 (&qf)[RT][NG],
+                                             float (&scale)[RT], int (&limit)[RT]) {
+  const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
     const int row = row0 + 16 * rt + i, token = fast_div(row, a.by_group), head = row - token * a.group;
@@ -314,7 +293,146 @@ __global__ void __launch_bounds__(kWaves * 64, RT == 1 ? 3 : 2) kv4_attn_kernel(
         qf[rt][s][2 * j + 1] = (f16)(a.scale < 0.0f ? -x[s][j + 4] : x[s][j + 4]);
       }
   }
+}
 
+// One tile's step of the running softmax.  acc: products of the lane's keys mine + 16 t + e (those of blocks
+// not in `there` and at or behind the row's limit are masked, if the tile has any), pf: weights as B operand of PV.
+template <int RT, int CT>
+__device__ __forceinline__ void softmax_tile(f32x4 (&acc)[RT][4], f32x4 (&o)[RT][CT], float (&top)[RT], float (&sum)[RT],
+                                             const float (&scale)[RT], const int (&limit)[RT], bool masked,
+                                             uint32_t there, int mine, f16x8 (&pf)[RT][2]) {
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    if (masked) {
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (!((there >> t) & 1) || mine + 16 * t + e >= limit[rt]) acc[rt][t][e] = -__builtin_inff();
+    }
+    float hi = -__builtin_inff();
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) hi = fmaxf(hi, acc[rt][t][e]);
+    hi = lanes16_max(hi) * scale[rt];
+    if (__any(hi > top[rt] + kKv4Slack)) {
+      const float up = fmaxf(hi, top[rt]), down = __builtin_amdgcn_exp2f(top[rt] - up);
+      top[rt] = up;
+      sum[rt] *= down;
+#pragma unroll
+      for (int ct = 0; ct < CT; ++ct) o[rt][ct] *= down;
+    }
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        acc[rt][t][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[rt][t][e], scale[rt], -top[rt]));
+        sum[rt] += acc[rt][t][e];
+      }
+#pragma unroll
+    for (int w = 0; w < 2; ++w)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        pf[rt][w][2 * e] = (f16)acc[rt][2 * w][e];
+        pf[rt][w][2 * e + 1] = (f16)acc[rt][2 * w + 1][e];
+      }
+  }
+}
+
+// Values that are not finite (a NaN was stored) are zeros in the products.  The rows that see such a key get a
+// NaN in its group's channels, the others must not (0 times NaN would be one).  broken[t]: bit 16 j + i
+// for group j of key 16 t + i.
+template <int NG, int RT, int CT>
+__device__ __forceinline__ void poison_rows(f32x4 (&o)[RT][CT], const uint64_t (&broken)[4], const int (&limit)[RT],
+                                            int key0) {
+  int at = 4 * ((threadIdx.x & 63) >> 4);
+  asm volatile("" : "+v"(at));  // what follows stays in this rare block
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    uint32_t seen = 0;  // groups
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      const uint32_t keys = (1u << min(max(limit[rt] - (key0 + 16 * t + at), 0), 4)) - 1;
+#pragma unroll
+      for (int j = 0; j < NG; ++j) {
+        const uint32_t bits = (uint32_t)(j < 2 ? broken[t] : broken[t] >> 32) >> (16 * (j & 1) + at);
+        seen |= (bits & keys) != 0 ? 1u << j : 0u;
+      }
+    }
+    seen = lanes16_or(seen);
+#pragma unroll
+    for (int ct = 0; ct < CT; ++ct)
+      if ((seen >> (ct >> 1)) & 1) o[rt][ct] = f32x4{} + __builtin_nanf("");
+  }
+}
+
+// Eight channels of a key: the word's codes with their group's scale and minimum.
+__device__ __forceinline__ f16x8 key_words(uint32_t word, uint32_t param) {
+  const f16x2 sm = __builtin_bit_cast(f16x2, param), sc = {sm[0], sm[0]}, mn = {sm[1], sm[1]};
+  f16x2 c[4];
+  kv4_codes(word, c);
+  f16x8 r;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const f16x2 v = kv4_fma(c[j], sc, mn);
+    r[2 * j] = v[0];
+    r[2 * j + 1] = v[1];
+  }
+  return r;
+}
+
+// Scales and minima of one group for the lane's 16 keys, as lds_s and lds_m hold them.
+struct ValueParams {
+  f16x8 s[2], m[2];
+  __device__ __forceinline__ ValueParams(const f16* lds_s, const f16* lds_m) {
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      s[w] = *reinterpret_cast<const f16x8*>(lds_s + 8 * w);
+      m[w] = *reinterpret_cast<const f16x8*>(lds_m + 8 * w);
+    }
+  }
+  // Word w of a channel: eight keys.
+  __device__ __forceinline__ f16x8 values(uint32_t word, int w) const {
+    f16x2 c[4];
+    kv4_codes(word, c);
+    f16x8 r;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const f16x2 v = kv4_fma(c[e], f16x2{s[w][2 * e], s[w][2 * e + 1]}, f16x2{m[w][2 * e], m[w][2 * e + 1]});
+      r[2 * e] = v[0];
+      r[2 * e + 1] = v[1];
+    }
+    return r;
+  }
+};
+
+template <int NG, int RT>
+__global__ void __launch_bounds__(kWaves * 64, RT == 1 ? 3 : 2) kv4_attn_kernel(const Kv4Args a) {
+  using Tile = Kv4Tile<NG>;
+  constexpr int kCT = 2 * NG;  // tiles of 16 channels
+  extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15,
+            g = lane >> 4;
+  const int rb = fast_div(blockIdx.x, a.by_splits), split = blockIdx.x - rb * a.splits;
+  const Kv4Item it = kv4_item(a, blockIdx.z, blockIdx.y, rb, 16 * RT);
+  const int row0 = rb * 16 * RT;
+  if (row0 >= it.rows) return;
+  const int tiles = it.kmax <= 0 ? 0 : (it.kmax + kTile - 1) / kTile;
+  const int first = split * a.split_tiles, last = min(tiles, first + a.split_tiles);
+  if (first >= last && split > 0) return;
+
+  // ---- the first keys' places are on their way while the queries come ----
+  Kv4Walk walk;
+  walk.table = a.table + it.b * a.s_table;
+  walk.key0 = (first + wave) * kTile;
+  walk.end = min(it.kmax, last * kTile);
+  walk.ids = walk.fetch(a, 0);
+
+  f16x8 qf[RT][NG];
+  float scale[RT];
+  int limit[RT];
+  load_queries(a, it, row0, qf, scale, limit);
   f32x4 o[RT][kCT];
   float top[RT], sum[RT];
 #pragma unroll
@@ -381,16 +499,7 @@ __global__ void __launch_bounds__(kWaves * 64, RT == 1 ? 3 : 2) kv4_attn_kernel(
 #pragma unroll
       for (int s = 0; s < NG; ++s) {
         const uint32_t p = NG == 3 && (NG * g + s) / 4 != NG * g / 4 ? x.kp[t][Tile::kNP - 1] : x.kp[t][0];
-        const f16x2 sm = __builtin_bit_cast(f16x2, p), sc = {sm[0], sm[0]}, mn = {sm[1], sm[1]};
-        f16x2 c[4];
-        kv4_codes(x.k[t][s], c);
-        f16x8 kf;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const f16x2 v = kv4_fma(c[j], sc, mn);
-          kf[2 * j] = v[0];
-          kf[2 * j + 1] = v[1];
-        }
+        const f16x8 kf = key_words(x.k[t][s], p);
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt)
           acc[rt][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[rt][s], acc[rt][t], 0, 0, 0);
@@ -408,60 +517,14 @@ __global__ void __launch_bounds__(kWaves * 64, RT == 1 ? 3 : 2) kv4_attn_kernel(
     // ---- softmax ----
     f16x8 pf[RT][2];
     const int mine = key0 + 4 * g;  // the lane's keys are mine + 16 t + e
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      if (masked) {
-#pragma unroll
-        for (int t = 0; t < 4; ++t)
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (!((here >> t) & 1) || mine + 16 * t + e >= limit[rt]) acc[rt][t][e] = -__builtin_inff();
-      }
-      float hi = -__builtin_inff();
-#pragma unroll
-      for (int t = 0; t < 4; ++t)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) hi = fmaxf(hi, acc[rt][t][e]);
-      hi = lanes16_max(hi) * scale[rt];
-      if (__any(hi > top[rt] + kKv4Slack)) {
-        const float up = fmaxf(hi, top[rt]), down = __builtin_amdgcn_exp2f(top[rt] - up);
-        top[rt] = up;
-        sum[rt] *= down;
-#pragma unroll
-        for (int ct = 0; ct < kCT; ++ct) o[rt][ct] *= down;
-      }
-#pragma unroll
-      for (int t = 0; t < 4; ++t)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          acc[rt][t][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[rt][t][e], scale[rt], -top[rt]));
-          sum[rt] += acc[rt][t][e];
-        }
-#pragma unroll
-      for (int w = 0; w < 2; ++w)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          pf[rt][w][2 * e] = (f16)acc[rt][2 * w][e];
-          pf[rt][w][2 * e + 1] = (f16)acc[rt][2 * w + 1][e];
-        }
-    }
+    softmax_tile(acc, o, top, sum, scale, limit, masked, here, mine, pf);
     // ---- O^T += V^T P^T ----
     const unsigned char* const v_tile = lds_v + (n & 1) * 4 * kBlockLds + v_at;
 #pragma unroll
     for (int j = 0; j < NG; ++j) {
       // (one group's parameters at a time: fetched all ahead they would take 64 registers)
       __builtin_amdgcn_sched_barrier(0);
-      f16x2 sc[8], mn[8];
-#pragma unroll
-      for (int w = 0; w < 2; ++w) {
-        const f16x8 s8 = *reinterpret_cast<const f16x8*>(lds_s + j * 64 + 16 * g + 8 * w);
-        const f16x8 m8 = *reinterpret_cast<const f16x8*>(lds_m + j * 64 + 16 * g + 8 * w);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          sc[4 * w + e] = f16x2{s8[2 * e], s8[2 * e + 1]};
-          mn[4 * w + e] = f16x2{m8[2 * e], m8[2 * e + 1]};
-        }
-      }
+      const ValueParams params(lds_s + j * 64 + 16 * g, lds_m + j * 64 + 16 * g);
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         const int ct = 2 * j + c;
@@ -469,15 +532,7 @@ __global__ void __launch_bounds__(kWaves * 64, RT == 1 ? 3 : 2) kv4_attn_kernel(
             (__attribute__((address_space(3))) i32x2*)(v_tile + 256 * j + 8 * c));
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
-          f16x2 code[4];
-          kv4_codes((uint32_t)words[w], code);
-          f16x8 vf;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const f16x2 v = kv4_fma(code[e], sc[4 * w + e], mn[4 * w + e]);
-            vf[2 * e] = v[0];
-            vf[2 * e + 1] = v[1];
-          }
+          const f16x8 vf = params.values((uint32_t)words[w], w);
 #pragma unroll
           for (int rt = 0; rt < RT; ++rt)
             o[rt][ct] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf, pf[rt][w], o[rt][ct], 0, 0, 0);
@@ -486,27 +541,7 @@ __global__ void __launch_bounds__(kWaves * 64, RT == 1 ? 3 : 2) kv4_attn_kernel(
     }
     // Values that are not finite (a NaN was stored): the rows that see the key get a NaN in the
     // group's channels, the others must not (0 times NaN would be one).
-    if (any_broken) {
-      int at = 4 * g;
-      asm volatile("" : "+v"(at));  // what follows stays in this rare block
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt) {
-        uint32_t seen = 0;  // groups
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          const uint32_t keys = (1u << min(max(limit[rt] - (key0 + 16 * t + at), 0), 4)) - 1;
-#pragma unroll
-          for (int j = 0; j < NG; ++j) {
-            const uint32_t bits = (uint32_t)(j < 2 ? broken[t] : broken[t] >> 32) >> (16 * (j & 1) + at);
-            seen |= (bits & keys) != 0 ? 1u << j : 0u;
-          }
-        }
-        seen = lanes16_or(seen);
-#pragma unroll
-        for (int ct = 0; ct < kCT; ++ct)
-          if ((seen >> (ct >> 1)) & 1) o[rt][ct] = f32x4{} + __builtin_nanf("");
-      }
-    }
+    if (any_broken) poison_rows<NG>(o, broken, limit, key0);
   }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no copy is left that could overwrite what follows
 
