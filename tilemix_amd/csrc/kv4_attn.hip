@@ -21,6 +21,7 @@ namespace {
 
 constexpr int kTile = 64;  // keys
 constexpr int kWaves = 4;
+constexpr int kChunkRT = 2, kChunkRows = kWaves * 16 * kChunkRT;  // query rows of a wave (in 16s), of a workgroup
 // The running maximum is raised when a row exceeds it by this much (in powers of two): most
 // tiles then leave the outputs unscaled.
 constexpr float kKv4Slack = 8.0f;
@@ -385,6 +386,7 @@ __device__ __forceinline__ f16x8 key_words(uint32_t word, uint32_t param) {
 // Scales and minima of one group for the lane's 16 keys, as lds_s and lds_m hold them.
 struct ValueParams {
   f16x8 s[2], m[2];
+  ValueParams() = default;
   __device__ __forceinline__ ValueParams(const f16* lds_s, const f16* lds_m) {
 #pragma unroll
     for (int w = 0; w < 2; ++w) {
@@ -592,6 +594,265 @@ __global__ void __launch_bounds__(kWaves * 64, RT == 1 ? 3 : 2) kv4_attn_kernel(
   }
 }
 
+// ---- many query rows ---------------------------------------------------------------
+// A workgroup takes 32 RT query rows, 16 RT of each wave, and all its waves go through the same
+// tiles: each turns a quarter of a tile's codes into fp16 operands, which all read from LDS as they
+// lie in the registers (operand [..][lane], no bank conflicts in either direction).
+// While tile n is multiplied, the operands of tile n + 1 are made and the codes of tile n + 2 are
+// on their way; one barrier a tile.  K's codes come in registers (wave t: block t), V's as copies to LDS,
+// from which wave t makes the channels ct = t and t + 4.
+template <int NG>
+struct ChunkLds {
+  f16x8 k[2][4 * NG * 64];      // [tile][(t NG + s) 64 + lane]
+  f16x8 v[2][4 * NG * 64];      // [tile][(2 ct + w) 64 + lane]
+  unsigned char codes[2][4 * kBlockLds];
+  f16 scale[2][NG * 64], least[2][NG * 64];
+  uint64_t broken[2][4];
+};
+
+template <int NG, int RT>
+__global__ void __launch_bounds__(kWaves * 64, 2) kv4_chunk_kernel(const Kv4Args a) {
+  constexpr int kCT = 2 * NG, kNP = Kv4Tile<NG>::kNP, kRows = kWaves * 16 * RT;
+  __shared__ __attribute__((aligned(16))) ChunkLds<NG> lds;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15,
+            g = lane >> 4;
+  const int rb = fast_div(blockIdx.y, a.by_splits), split = blockIdx.y - rb * a.splits;
+  const Kv4Item it = kv4_item(a, blockIdx.z, blockIdx.x, rb, kRows);
+  if (rb * kRows >= it.rows) return;
+  const int tiles = it.kmax <= 0 ? 0 : (it.kmax + kTile - 1) / kTile;
+  const int first = split * a.split_tiles, last = min(tiles, first + a.split_tiles);
+  if (first >= last && split > 0) return;
+  const int end = min(it.kmax, last * kTile);  // keys
+
+  // The rows of the pool of block t of the tiles first + 64 c .. + 63, one in each lane (-1: no page).
+  const int32_t* const table = a.table + it.b * a.s_table;
+  auto fetch = [&](int n, int t) {
+    const int key = (first + n + lane) * kTile + 16 * t;
+    return key < end ? table[fast_div(key, a.by_page)] : -1;
+  };
+  int ids[4];
+#pragma unroll
+  for (int t = 0; t < 4; ++t) ids[t] = fetch(0, t);
+
+  const int row0 = rb * kRows + wave * 16 * RT;  // of the wave
+  f16x8 qf[RT][NG];
+  float scale[RT];
+  int limit[RT];
+  load_queries(a, it, min(row0, it.rows - 1), qf, scale, limit);
+  const bool rows_there = row0 < it.rows;
+  // keys that the wave's first row and its last one see
+  const int all_see = it.limit0 + (a.causal ? fast_div(row0, a.by_group) : 0);
+  const int some_see = it.limit0 + (a.causal ? fast_div(min(row0 + 16 * RT, it.rows) - 1, a.by_group) : 0);
+
+  f32x4 o[RT][kCT];
+  float top[RT], sum[RT];
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    top[rt] = kNoKey;
+    sum[rt] = 0.0f;
+#pragma unroll
+    for (int ct = 0; ct < kCT; ++ct) o[rt][ct] = f32x4{};
+  }
+
+  // ---- loads ----
+  const int gc = g < NG ? g : NG - 1;
+  const uint32_t words_at = i * (4 * NG) + NG * g, chunk_at = 16 * (i * NG + gc), group_at = i * NG + gc;
+  const uint32_t codes_lds = lds_addr(&lds.codes[0][0]) + wave * kBlockLds;
+  uint64_t pages[4];  // bit n % 64: block t of tile n has a page
+  int rows = 0;
+  struct KeyCodes {
+    uint32_t k[NG], kp[kNP];
+  } fresh, codes;  // of the tile that is loaded, and of the one that is made
+  uint32_t vp;
+  auto start = [&](int n) {  // tile n's codes; which of its blocks have a page
+    if ((n & 63) == 0) {
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const bool ok = ids[t] >= 0 && ids[t] < a.pages;
+        pages[t] = __ballot(ok);
+        if (t == wave) {
+          const int key = (first + n + lane) * kTile + 16 * t, column = fast_div(key, a.by_page);
+          rows = ok ? (ids[t] * a.hk + it.h) * a.by_page.d + (key - column * a.by_page.d) : 0;
+        }
+        ids[t] = fetch(n + 64, t);
+      }
+    }
+    uint32_t there = 0;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) there |= (uint32_t)((pages[t] >> (n & 63)) & 1) << t;
+    const int64_t row = __builtin_amdgcn_readlane(rows, n & 63);
+    copy16(a.vc + row * (4 * NG), chunk_at, codes_lds + (n & 1) * 4 * kBlockLds);
+    load_words(fresh.k, a.kc + row * (4 * NG) + words_at);
+#pragma unroll
+    for (int j = 0; j < kNP; ++j) {
+      const uint32_t group = NG == 4 ? g : j == 0 ? NG * g / 4 : (NG * g + NG - 1) / 4;
+      fresh.kp[j] = (a.kp + row * NG)[i * NG + group];
+    }
+    vp = (a.vp + row * NG)[group_at];
+    return there;
+  };
+  // V's parameters of tile n (in vp) to LDS, in the order of the pairs
+  const int p_at = 16 * (i >> 2) + 2 * (i & 3) + 8 * (wave >> 1) + (wave & 1);
+  auto stage_params = [&](int n, uint32_t there) {
+    uint32_t p = vp;
+    if (!((there >> wave) & 1) || (first + n) * kTile + 16 * wave + i >= end) p = 0;
+    const uint64_t bad = __ballot(kv4_not_finite(p));
+    if (kv4_not_finite(p)) p = 0;
+    const f16x2 sm = __builtin_bit_cast(f16x2, p);
+    if (NG == 4 || g < NG) {
+      lds.scale[n & 1][g * 64 + p_at] = sm[0];
+      lds.least[n & 1][g * 64 + p_at] = sm[1];
+    }
+    if (lane == 0) lds.broken[n & 1][wave] = bad;
+  };
+  auto make_k = [&](int n, int s) {  // one word of each key
+    const uint32_t p = NG == 3 && (NG * g + s) / 4 != NG * g / 4 ? codes.kp[kNP - 1] : codes.kp[0];
+    lds.k[n & 1][(wave * NG + s) * 64 + lane] = key_words(codes.k[s], p);
+  };
+  const int v_at = (i >> 2) * kBlockLds + (4 * g + (i & 3)) * 16;
+  // 16 channels ct = wave + 4 c: reads and conversion apart, so that products fit between them
+  auto has_v = [&](int c) { return NG == 4 || wave + 4 * c < kCT; };
+  auto read_v = [&](int n, int c, i32x2& words) {
+    const int ct = wave + 4 * c, j = ct >> 1;
+    words = __builtin_amdgcn_ds_read_tr4_b64_v2i32(
+        (__attribute__((address_space(3))) i32x2*)(lds.codes[n & 1] + v_at + 256 * j + 8 * (ct & 1)));
+    return ValueParams(lds.scale[n & 1] + j * 64 + 16 * g, lds.least[n & 1] + j * 64 + 16 * g);
+  };
+  auto write_v = [&](int n, int c, const i32x2& words, const ValueParams& params) {
+#pragma unroll
+    for (int w = 0; w < 2; ++w)
+      lds.v[n & 1][(2 * (wave + 4 * c) + w) * 64 + lane] = params.values((uint32_t)words[w], w);
+  };
+  auto make_v = [&](int n, int c) {
+    if (has_v(c)) {
+      i32x2 words;
+      const ValueParams params = read_v(n, c, words);
+      write_v(n, c, words, params);
+    }
+  };
+
+  // ---- tile 0 is made, tile 1 has been loaded ----
+  const int count = last - first;
+  uint32_t there[3];  // of tiles n, n + 1, n + 2
+  there[0] = start(0);
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  stage_params(0, there[0]);
+  codes = fresh;
+#pragma unroll
+  for (int s = 0; s < NG; ++s) make_k(0, s);
+  __syncthreads();
+#pragma unroll
+  for (int c = 0; c < 2; ++c) make_v(0, c);
+  uint64_t broken[4];
+#pragma unroll
+  for (int t = 0; t < 4; ++t) broken[t] = lds.broken[0][t];
+  there[1] = start(1);
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  stage_params(1, there[1]);
+  codes = fresh;
+  __syncthreads();
+
+  for (int n = 0; n < count; ++n) {
+    const int key0 = (first + n) * kTile;
+    there[2] = start(n + 2);
+    uint64_t broken_next[4];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) broken_next[t] = lds.broken[(n + 1) & 1][t];
+    if (rows_there && key0 < some_see) {
+      // The operands of a step are read one step ahead, and the next tile's are made in the shadow of
+      // the products (the barriers keep the compiler from moving the reads back to their uses).
+      const f16x8* const kf = lds.k[n & 1] + lane;
+      const f16x8* const vf = lds.v[n & 1] + lane;
+      f32x4 acc[RT][4];
+      f16x8 x[2][4];
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        x[0][t] = kf[t * NG * 64];
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) acc[rt][t] = f32x4{};
+      }
+#pragma unroll
+      for (int s = 0; s < NG; ++s) {
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) x[(s + 1) & 1][t] = s + 1 < NG ? kf[(t * NG + s + 1) * 64] : vf[t * 64];
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt)
+            acc[rt][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[s & 1][t], qf[rt][s], acc[rt][t], 0, 0, 0);
+        make_k(n + 1, s);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      const bool masked = key0 + kTile > all_see || there[0] != 15u;
+      f16x8 pf[RT][2];
+      softmax_tile(acc, o, top, sum, scale, limit, masked, there[0], key0 + 4 * g, pf);
+      // V's operands 4 c .. 4 c + 3 are the channels 2 c and 2 c + 1 of 16, two words each
+#pragma unroll
+      for (int c = 0; c < NG; ++c) {
+        const int at = (NG + c) & 1;
+        __builtin_amdgcn_sched_barrier(0);
+        if (c + 1 < NG) {
+#pragma unroll
+          for (int t = 0; t < 4; ++t) x[at ^ 1][t] = vf[(4 * (c + 1) + t) * 64];
+        }
+        i32x2 words;
+        ValueParams params;
+        if (NG == 4 && c < 2) params = read_v(n + 1, c, words);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt)
+            o[rt][2 * c + (t >> 1)] =
+                __builtin_amdgcn_mfma_f32_16x16x32_f16(x[at][t], pf[rt][t & 1], o[rt][2 * c + (t >> 1)], 0, 0, 0);
+        if (NG == 4 && c < 2) write_v(n + 1, c, words, params);
+      }
+      if (NG < 4) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c) make_v(n + 1, c);
+      }
+      if ((broken[0] | broken[1] | broken[2] | broken[3]) != 0) poison_rows<NG>(o, broken, limit, key0);
+    } else {
+#pragma unroll
+      for (int s = 0; s < NG; ++s) make_k(n + 1, s);
+#pragma unroll
+      for (int c = 0; c < 2; ++c) make_v(n + 1, c);
+    }
+    // tile n + 2 has arrived; its parameters take the place of tile n's, whose operands all waves have made
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    stage_params(n + 2, there[2]);
+    codes = fresh;
+    there[0] = there[1];
+    there[1] = there[2];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) broken[t] = broken_next[t];
+    __syncthreads();
+  }
+
+  // ---- each wave has its rows for itself ----
+  if (!rows_there) return;
+  const int64_t item = ((int64_t)(it.b * a.hk + it.h) * a.row_blocks + rb) * a.splits + split;
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    const float all = lanes16_sum(sum[rt]);
+    const int row = row0 + 16 * rt + i, token = fast_div(row, a.by_group), head = row - token * a.group;
+    if (row >= it.rows) continue;
+    const int64_t part = item * kRows + wave * 16 * RT + 16 * rt + i;
+    if (a.splits > 1 && g == 0) a.part_ml[part] = make_float2(top[rt], all);
+    const float norm = all == 0.0f ? 0.0f : 1.0f / all;
+#pragma unroll
+    for (int ct = 0; ct < kCT; ++ct) {
+      const int c = 16 * ct + 4 * g;
+      if (a.splits > 1) *reinterpret_cast<f32x4*>(a.part + part * (32 * NG) + c) = o[rt][ct];
+      else
+        store_out(a.out, (it.start + token) * a.so_t + (it.h * a.group + head) * a.so_h + c, o[rt][ct] * norm, a.d - c,
+                  a.o_vec, a.bf);
+    }
+  }
+}
+
 // Adds up the splits of a row.  One thread takes four channels of every `lanes`-th split and keeps
 // its own running maximum; the `lanes` threads of a row's channels meet in LDS.
 template <int NG>
@@ -644,7 +905,7 @@ __global__ void __launch_bounds__(256) kv4_join_kernel(const Kv4Args a, int bloc
 }
 
 struct Plan {
-  int rt, row_blocks, splits, split_tiles;
+  int block_rows, row_blocks, splits, split_tiles;
   int64_t bytes;
 };
 
@@ -659,17 +920,17 @@ bool make_plan(const char* what, const tilemix_kv4_attn_params& p, Plan& plan) {
     return false;
   }
   const int64_t rows = (int64_t)p.max_seqlen_q * (p.heads_q / p.heads_k);
-  plan.rt = rows <= 16 ? 1 : 2;
-  const int64_t blocks = (rows + 16 * plan.rt - 1) / (16 * plan.rt);
+  plan.block_rows = rows <= 16 ? 16 : rows <= 32 ? 32 : kChunkRows;
+  const int64_t blocks = (rows + plan.block_rows - 1) / plan.block_rows;
   const int64_t keys = std::min<int64_t>(p.max_seqlen_k, (int64_t)p.table_columns * p.page_size);
   const int64_t tiles = std::max<int64_t>((keys + kTile - 1) / kTile, 1);
   const int64_t items = std::max<int64_t>(blocks * p.heads_k * p.batch, 1);
-  const int64_t wanted = std::max<int64_t>(1, (int64_t)1024 / items);
+  const int64_t wanted = std::max<int64_t>(1, (int64_t)(plan.block_rows < kChunkRows ? 1024 : 512) / items);
   int64_t split_tiles = (tiles + wanted - 1) / wanted;
   split_tiles = (split_tiles + kWaves - 1) / kWaves * kWaves;
   const int64_t splits = (tiles + split_tiles - 1) / split_tiles;
   const int64_t grid = blocks * splits;
-  if (rows > INT32_MAX || grid > (1 << 24) - 1 || items * splits > INT32_MAX / 64) {
+  if (rows > INT32_MAX / 2 || grid > (plan.block_rows < kChunkRows ? (1 << 24) - 1 : 65535) || items * splits > INT32_MAX / 64) {
     set_error("%s: too many queries for one call (%lld rows a sequence, batch %d)", what, (long long)rows, p.batch);
     return false;
   }
@@ -677,30 +938,31 @@ bool make_plan(const char* what, const tilemix_kv4_attn_params& p, Plan& plan) {
   plan.splits = (int)splits;
   plan.split_tiles = (int)split_tiles;
   const int width = (p.head_dim + kKv4Group - 1) / kKv4Group * kKv4Group;
-  plan.bytes = splits > 1 ? items * splits * 16 * plan.rt * (width * 4 + 8) : 0;
+  plan.bytes = splits > 1 ? items * splits * plan.block_rows * (width * 4 + 8) : 0;
   return true;
 }
 
-template <int NG, int RT>
-void launch_kv4(const Kv4Args& a, int batch, hipStream_t stream) {
-  constexpr int lds = kv4_lds_bytes<NG, RT>();
-  hipLaunchKernelGGL((kv4_attn_kernel<NG, RT>), dim3((unsigned)(a.row_blocks * a.splits), a.hk, batch),
-                     dim3(kWaves * 64), lds, stream, a);
+template <int NG>
+void launch_kv4(const Kv4Args& a, int block_rows, int batch, hipStream_t stream) {
+  if (block_rows < kChunkRows) {
+    const dim3 grid((unsigned)(a.row_blocks * a.splits), a.hk, batch), block(kWaves * 64);
+    constexpr int lds1 = kv4_lds_bytes<NG, 1>(), lds2 = kv4_lds_bytes<NG, 2>();
+    if (block_rows == 16) hipLaunchKernelGGL((kv4_attn_kernel<NG, 1>), grid, block, lds1, stream, a);
+    else hipLaunchKernelGGL((kv4_attn_kernel<NG, 2>), grid, block, lds2, stream, a);
+  } else {
+    // Heads are the fastest: the workgroups of a head, which read the same keys, meet on few XCDs.
+    hipLaunchKernelGGL((kv4_chunk_kernel<NG, kChunkRT>), dim3(a.hk, (unsigned)(a.row_blocks * a.splits), batch),
+                       dim3(kWaves * 64), 0, stream, a);
+  }
   if (a.splits > 1) {
     // about four splits a thread
     constexpr int units = 256 / (8 * NG);
     int lanes = 1;
     while (lanes * 2 <= units && lanes * 4 < a.splits) lanes *= 2;
     const int rows = units / lanes;
-    hipLaunchKernelGGL((kv4_join_kernel<NG>), dim3((unsigned)(a.row_blocks * ((16 * RT + rows - 1) / rows)), a.hk, batch),
-                       dim3(256), 0, stream, a, 16 * RT, lanes, rows);
+    const dim3 grid((unsigned)(a.row_blocks * ((block_rows + rows - 1) / rows)), a.hk, batch);
+    hipLaunchKernelGGL((kv4_join_kernel<NG>), grid, dim3(256), 0, stream, a, block_rows, lanes, rows);
   }
-}
-
-template <int NG>
-void launch_kv4(const Kv4Args& a, int rt, int batch, hipStream_t stream) {
-  if (rt == 1) launch_kv4<NG, 1>(a, batch, stream);
-  else launch_kv4<NG, 2>(a, batch, stream);
 }
 
 }  // namespace
@@ -738,7 +1000,7 @@ int launch_kv4_attn(const tilemix_kv4_attn_params& p, hipStream_t stream) {
   a.lens = p.seq_lens;
   a.cu = p.cu_seqlens_q;
   a.part = static_cast<float*>(p.workspace);
-  const int64_t parts = (int64_t)p.batch * p.heads_k * plan.row_blocks * plan.splits * 16 * plan.rt;
+  const int64_t parts = (int64_t)p.batch * p.heads_k * plan.row_blocks * plan.splits * plan.block_rows;
   if (plan.bytes > 0) a.part_ml = reinterpret_cast<float2*>(a.part + parts * width);
   a.sq_t = p.stride_q_token;
   a.sq_h = p.stride_q_head;
@@ -767,16 +1029,16 @@ int launch_kv4_attn(const tilemix_kv4_attn_params& p, hipStream_t stream) {
   a.by_splits = make_fast_div(a.splits);
   switch (width / kKv4Group) {
     case 1:
-      launch_kv4<1>(a, plan.rt, p.batch, stream);
+      launch_kv4<1>(a, plan.block_rows, p.batch, stream);
       break;
     case 2:
-      launch_kv4<2>(a, plan.rt, p.batch, stream);
+      launch_kv4<2>(a, plan.block_rows, p.batch, stream);
       break;
     case 3:
-      launch_kv4<3>(a, plan.rt, p.batch, stream);
+      launch_kv4<3>(a, plan.block_rows, p.batch, stream);
       break;
     default:
-      launch_kv4<4>(a, plan.rt, p.batch, stream);
+      launch_kv4<4>(a, plan.block_rows, p.batch, stream);
   }
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) {
