@@ -10,7 +10,7 @@
 //   p = exp2(S^T c - M)  c = sm_scale log2(e), M the row's running maximum
 //   O^T += V^T P^T       channels x rows
 // p is rounded to fp16 for the second product (p <= 2^8, see kKv4Slack; relative error 2^-11,
-// as small as the output's own rounding), the row sum adds the unrounded p.
+// as small as the output's own rounding), and the row sum adds the same rounded weights.
 #include "kv4_common.h"
 
 #include <algorithm>
@@ -85,12 +85,6 @@ __device__ __forceinline__ float lanes16_max(float x) {
   x = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
   const float2 h = swap_halves(x);
   return fmaxf(h.x, h.y);
-}
-__device__ __forceinline__ float lanes16_sum(float x) {
-  auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  x = __uint_as_float(r[0]) + __uint_as_float(r[1]);
-  const float2 h = swap_halves(x);
-  return h.x + h.y;
 }
 __device__ __forceinline__ uint32_t lanes16_or(uint32_t x) {
   auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
@@ -296,49 +290,52 @@ __device__ __forceinline__ void load_queries(const Kv4Args& a, const Kv4Item& it
   }
 }
 
-// One tile's step of the running softmax.  acc: products of the lane's keys mine + 16 t + e (those of blocks
-// not in `there` and at or behind the row's limit are masked, if the tile has any), pf: weights as B operand of PV.
-template <int RT, int CT>
-__device__ __forceinline__ void softmax_tile(f32x4 (&acc)[RT][4], f32x4 (&o)[RT][CT], float (&top)[RT], float (&sum)[RT],
-                                             const float (&scale)[RT], const int (&limit)[RT], bool masked,
-                                             uint32_t there, int mine, f16x8 (&pf)[RT][2]) {
+// The running softmax of a row tile, in two steps.  acc: products of the lane's keys mine + 16 t + e.  First the
+// maximum (keys of blocks not in `there` and at or behind the row's limit are masked, if the tile has any).
+__device__ __forceinline__ void mask_tile(f32x4 (&acc)[4], int limit, uint32_t there, int mine) {
 #pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-    if (masked) {
+  for (int t = 0; t < 4; ++t)
 #pragma unroll
-      for (int t = 0; t < 4; ++t)
+    for (int e = 0; e < 4; ++e)
+      if (!((there >> t) & 1) || mine + 16 * t + e >= limit) acc[t][e] = -__builtin_inff();
+}
+__device__ __forceinline__ float tile_max(const f32x4 (&acc)[4], float scale) {
+  float hi = -__builtin_inff();
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (!((there >> t) & 1) || mine + 16 * t + e >= limit[rt]) acc[rt][t][e] = -__builtin_inff();
-    }
-    float hi = -__builtin_inff();
+  for (int t = 0; t < 4; ++t)
 #pragma unroll
-    for (int t = 0; t < 4; ++t)
+    for (int e = 0; e < 4; ++e) hi = fmaxf(hi, acc[t][e]);
+  return lanes16_max(hi) * scale;
+}
+// Raises the running maximum where a row needs it.
+template <int CT>
+__device__ __forceinline__ void raise_max(float hi, float& top, f32x4& sum, f32x4 (&o)[CT]) {
+  if (__any(hi > top + kKv4Slack)) {
+    const float up = fmaxf(hi, top), down = __builtin_amdgcn_exp2f(top - up);
+    top = up;
+    sum *= down;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) hi = fmaxf(hi, acc[rt][t][e]);
-    hi = lanes16_max(hi) * scale[rt];
-    if (__any(hi > top[rt] + kKv4Slack)) {
-      const float up = fmaxf(hi, top[rt]), down = __builtin_amdgcn_exp2f(top[rt] - up);
-      top[rt] = up;
-      sum[rt] *= down;
-#pragma unroll
-      for (int ct = 0; ct < CT; ++ct) o[rt][ct] *= down;
-    }
-#pragma unroll
-    for (int t = 0; t < 4; ++t)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        acc[rt][t][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[rt][t][e], scale[rt], -top[rt]));
-        sum[rt] += acc[rt][t][e];
-      }
-#pragma unroll
-    for (int w = 0; w < 2; ++w)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        pf[rt][w][2 * e] = (f16)acc[rt][2 * w][e];
-        pf[rt][w][2 * e + 1] = (f16)acc[rt][2 * w + 1][e];
-      }
+    for (int ct = 0; ct < CT; ++ct) o[ct] *= down;
   }
+}
+// Then the weights, as B operand of PV.
+__device__ __forceinline__ void tile_weights(const f32x4 (&acc)[4], float scale, float top, f16x8 (&pf)[2]) {
+#pragma unroll
+  for (int w = 0; w < 2; ++w)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      pf[w][2 * e] = (f16)__builtin_amdgcn_exp2f(__builtin_fmaf(acc[2 * w][e], scale, -top));
+      pf[w][2 * e + 1] = (f16)__builtin_amdgcn_exp2f(__builtin_fmaf(acc[2 * w + 1][e], scale, -top));
+    }
+}
+// The row sums of the weights, on the matrix pipe: sixteen rows of ones (each result row is the sum).
+__device__ __forceinline__ f32x4 add_weights(const f16x8 (&pf)[2], f32x4 sum) {
+  f16x8 ones;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) ones[e] = (f16)1.0f;
+#pragma unroll
+  for (int w = 0; w < 2; ++w) sum = __builtin_amdgcn_mfma_f32_16x16x32_f16(ones, pf[w], sum, 0, 0, 0);
+  return sum;
 }
 
 // Values that are not finite (a NaN was stored) are zeros in the products.  The rows that see such a key get a
@@ -436,11 +433,12 @@ __global__ void __launch_bounds__(kWaves * 64, RT == 1 ? 3 : 2) kv4_attn_kernel(
   int limit[RT];
   load_queries(a, it, row0, qf, scale, limit);
   f32x4 o[RT][kCT];
-  float top[RT], sum[RT];
+  float top[RT];
+  f32x4 sum[RT];  // four times the same
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
     top[rt] = kNoKey;
-    sum[rt] = 0.0f;
+    sum[rt] = f32x4{};
 #pragma unroll
     for (int ct = 0; ct < kCT; ++ct) o[rt][ct] = f32x4{};
   }
@@ -519,7 +517,13 @@ __global__ void __launch_bounds__(kWaves * 64, RT == 1 ? 3 : 2) kv4_attn_kernel(
     // ---- softmax ----
     f16x8 pf[RT][2];
     const int mine = key0 + 4 * g;  // the lane's keys are mine + 16 t + e
-    softmax_tile(acc, o, top, sum, scale, limit, masked, here, mine, pf);
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      if (masked) mask_tile(acc[rt], limit[rt], here, mine);
+      raise_max(tile_max(acc[rt], scale[rt]), top[rt], sum[rt], o[rt]);
+      tile_weights(acc[rt], scale[rt], top[rt], pf[rt]);
+      sum[rt] = add_weights(pf[rt], sum[rt]);
+    }
     // ---- O^T += V^T P^T ----
     const unsigned char* const v_tile = lds_v + (n & 1) * 4 * kBlockLds + v_at;
 #pragma unroll
@@ -551,8 +555,7 @@ __global__ void __launch_bounds__(kWaves * 64, RT == 1 ? 3 : 2) kv4_attn_kernel(
   float2* const lds_ml = reinterpret_cast<float2*>(smem + kv4_lds_bytes<NG, RT>() - kWaves * RT * 16 * 8);
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
-    sum[rt] = lanes16_sum(sum[rt]);
-    if (g == 0) lds_ml[(wave * RT + rt) * 16 + i] = make_float2(top[rt], sum[rt]);
+    if (g == 0) lds_ml[(wave * RT + rt) * 16 + i] = make_float2(top[rt], sum[rt][0]);
   }
   const int item = ((it.b * a.hk + it.h) * a.row_blocks + rb) * a.splits + split;
   f32x4* const lds_o = reinterpret_cast<f32x4*>(smem);
@@ -598,17 +601,33 @@ __global__ void __launch_bounds__(kWaves * 64, RT == 1 ? 3 : 2) kv4_attn_kernel(
 // A workgroup takes 32 RT query rows, 16 RT of each wave, and all its waves go through the same
 // tiles: each turns a quarter of a tile's codes into fp16 operands, which all read from LDS as they
 // lie in the registers (operand [..][lane], no bank conflicts in either direction).
-// While tile n is multiplied, the operands of tile n + 1 are made and the codes of tile n + 2 are
-// on their way; one barrier a tile.  K's codes come in registers (wave t: block t), V's as copies to LDS,
-// from which wave t makes the channels ct = t and t + 4.
+// The loop is skewed so that the matrix pipe and the vector units have independent work side by side:
+// iteration n multiplies Q with the keys of tile n + 1 beside the softmax of tile n, then its weights with
+// the values of tile n beside the conversion of K's tile n + 2 and V's tile n + 1; the codes after those are
+// on their way.  One barrier a tile.  K's codes come in registers (wave t: block t), V's as copies to
+// LDS, from which wave t makes the channels ct = t and t + 4.
 template <int NG>
 struct ChunkLds {
   f16x8 k[2][4 * NG * 64];      // [tile][(t NG + s) 64 + lane]
   f16x8 v[2][4 * NG * 64];      // [tile][(2 ct + w) 64 + lane]
   unsigned char codes[2][4 * kBlockLds];
   f16 scale[2][NG * 64], least[2][NG * 64];
-  uint64_t broken[2][4];
+  // Of the tiles n, n + 1, ..: flags[n % 4][t] of block t: 1 it has a page, 2 it has values that are not finite,
+  // those of `broken` (poison_rows).
+  uint32_t flags[4][4];
+  uint64_t broken[4][4];
 };
+
+// Asks the scheduler for COUNT matrix instructions with VALU vector and TRANS transcendental ones behind each.
+template <int COUNT, int VALU, int TRANS>
+__device__ __forceinline__ void interleave() {
+#pragma unroll
+  for (int k = 0; k < COUNT; ++k) {
+    __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+    if (VALU > 0) __builtin_amdgcn_sched_group_barrier(0x2, VALU, 0);
+    if (TRANS > 0) __builtin_amdgcn_sched_group_barrier(0x400, TRANS, 0);
+  }
+}
 
 template <int NG, int RT>
 __global__ void __launch_bounds__(kWaves * 64, 2) kv4_chunk_kernel(const Kv4Args a) {
@@ -624,15 +643,13 @@ __global__ void __launch_bounds__(kWaves * 64, 2) kv4_chunk_kernel(const Kv4Args
   if (first >= last && split > 0) return;
   const int end = min(it.kmax, last * kTile);  // keys
 
-  // The rows of the pool of block t of the tiles first + 64 c .. + 63, one in each lane (-1: no page).
+  // The rows of the pool of block `wave` of the tiles first + 64 c .. + 63, one in each lane (-1: no page).
   const int32_t* const table = a.table + it.b * a.s_table;
-  auto fetch = [&](int n, int t) {
-    const int key = (first + n + lane) * kTile + 16 * t;
+  auto fetch = [&](int n) {
+    const int key = (first + n + lane) * kTile + 16 * wave;
     return key < end ? table[fast_div(key, a.by_page)] : -1;
   };
-  int ids[4];
-#pragma unroll
-  for (int t = 0; t < 4; ++t) ids[t] = fetch(0, t);
+  int ids = fetch(0), rows = -1;
 
   const int row0 = rb * kRows + wave * 16 * RT;  // of the wave
   f16x8 qf[RT][NG];
@@ -640,16 +657,15 @@ __global__ void __launch_bounds__(kWaves * 64, 2) kv4_chunk_kernel(const Kv4Args
   int limit[RT];
   load_queries(a, it, min(row0, it.rows - 1), qf, scale, limit);
   const bool rows_there = row0 < it.rows;
-  // keys that the wave's first row and its last one see
-  const int all_see = it.limit0 + (a.causal ? fast_div(row0, a.by_group) : 0);
-  const int some_see = it.limit0 + (a.causal ? fast_div(min(row0 + 16 * RT, it.rows) - 1, a.by_group) : 0);
+  const int all_see = it.limit0 + (a.causal ? fast_div(row0, a.by_group) : 0);  // keys that all rows of the wave see
 
   f32x4 o[RT][kCT];
-  float top[RT], sum[RT];
+  float top[RT];
+  f32x4 sum[RT];  // four times the same
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
     top[rt] = kNoKey;
-    sum[rt] = 0.0f;
+    sum[rt] = f32x4{};
 #pragma unroll
     for (int ct = 0; ct < kCT; ++ct) o[rt][ct] = f32x4{};
   }
@@ -658,52 +674,49 @@ __global__ void __launch_bounds__(kWaves * 64, 2) kv4_chunk_kernel(const Kv4Args
   const int gc = g < NG ? g : NG - 1;
   const uint32_t words_at = i * (4 * NG) + NG * g, chunk_at = 16 * (i * NG + gc), group_at = i * NG + gc;
   const uint32_t codes_lds = lds_addr(&lds.codes[0][0]) + wave * kBlockLds;
-  uint64_t pages[4];  // bit n % 64: block t of tile n has a page
-  int rows = 0;
   struct KeyCodes {
     uint32_t k[NG], kp[kNP];
   } fresh, codes;  // of the tile that is loaded, and of the one that is made
   uint32_t vp;
-  auto start = [&](int n) {  // tile n's codes; which of its blocks have a page
+  auto find = [&](int n) {  // the row of the wave's block of tile n
     if ((n & 63) == 0) {
-#pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        const bool ok = ids[t] >= 0 && ids[t] < a.pages;
-        pages[t] = __ballot(ok);
-        if (t == wave) {
-          const int key = (first + n + lane) * kTile + 16 * t, column = fast_div(key, a.by_page);
-          rows = ok ? (ids[t] * a.hk + it.h) * a.by_page.d + (key - column * a.by_page.d) : 0;
-        }
-        ids[t] = fetch(n + 64, t);
-      }
+      const int key = (first + n + lane) * kTile + 16 * wave, column = fast_div(key, a.by_page);
+      rows = ids >= 0 && ids < a.pages ? (ids * a.hk + it.h) * a.by_page.d + (key - column * a.by_page.d) : -1;
+      ids = fetch(n + 64);
     }
-    uint32_t there = 0;
-#pragma unroll
-    for (int t = 0; t < 4; ++t) there |= (uint32_t)((pages[t] >> (n & 63)) & 1) << t;
-    const int64_t row = __builtin_amdgcn_readlane(rows, n & 63);
-    copy16(a.vc + row * (4 * NG), chunk_at, codes_lds + (n & 1) * 4 * kBlockLds);
+    return __builtin_amdgcn_readlane(rows, n & 63);
+  };
+  auto load_k = [&](int found) {  // (a block without a page reads rows of page 0: they count for nothing)
+    const int64_t row = max(found, 0);
     load_words(fresh.k, a.kc + row * (4 * NG) + words_at);
 #pragma unroll
     for (int j = 0; j < kNP; ++j) {
       const uint32_t group = NG == 4 ? g : j == 0 ? NG * g / 4 : (NG * g + NG - 1) / 4;
       fresh.kp[j] = (a.kp + row * NG)[i * NG + group];
     }
+  };
+  auto load_v = [&](int n, int found) {
+    const int64_t row = max(found, 0);
+    copy16(a.vc + row * (4 * NG), chunk_at, codes_lds + (n & 1) * 4 * kBlockLds);
     vp = (a.vp + row * NG)[group_at];
-    return there;
   };
   // V's parameters of tile n (in vp) to LDS, in the order of the pairs
   const int p_at = 16 * (i >> 2) + 2 * (i & 3) + 8 * (wave >> 1) + (wave & 1);
-  auto stage_params = [&](int n, uint32_t there) {
+  auto stage_params = [&](int n, int found) {
     uint32_t p = vp;
-    if (!((there >> wave) & 1) || (first + n) * kTile + 16 * wave + i >= end) p = 0;
-    const uint64_t bad = __ballot(kv4_not_finite(p));
-    if (kv4_not_finite(p)) p = 0;
+    if (found < 0 || (first + n) * kTile + 16 * wave + i >= end) p = 0;
+    const bool bad = kv4_not_finite(p);
+    const uint64_t broken = __ballot(bad);
+    if (bad) p = 0;
     const f16x2 sm = __builtin_bit_cast(f16x2, p);
     if (NG == 4 || g < NG) {
       lds.scale[n & 1][g * 64 + p_at] = sm[0];
       lds.least[n & 1][g * 64 + p_at] = sm[1];
     }
-    if (lane == 0) lds.broken[n & 1][wave] = bad;
+    if (lane == 0) {
+      lds.flags[n & 3][wave] = (found >= 0 ? 1u : 0u) | (broken != 0 ? 2u : 0u);
+      lds.broken[n & 3][wave] = broken;
+    }
   };
   auto make_k = [&](int n, int s) {  // one word of each key
     const uint32_t p = NG == 3 && (NG * g + s) / 4 != NG * g / 4 ? codes.kp[kNP - 1] : codes.kp[0];
@@ -731,103 +744,145 @@ __global__ void __launch_bounds__(kWaves * 64, 2) kv4_chunk_kernel(const Kv4Args
     }
   };
 
-  // ---- tile 0 is made, tile 1 has been loaded ----
+  // ---- before tile 0: its scores, its values, K's tile 1, the codes of K's tile 2 and V's tile 1 ----
   const int count = last - first;
-  uint32_t there[3];  // of tiles n, n + 1, n + 2
-  there[0] = start(0);
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  stage_params(0, there[0]);
+  int row[3];  // of the wave's block of tiles n + 1 .. n + 3
+  auto wait_loads = [] { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); };
+  row[1] = find(0);
+  load_k(row[1]);
+  load_v(0, row[1]);
+  row[0] = find(1);
+  wait_loads();
+  stage_params(0, row[1]);
   codes = fresh;
+  load_k(row[0]);
 #pragma unroll
   for (int s = 0; s < NG; ++s) make_k(0, s);
   __syncthreads();
+  load_v(1, row[0]);
+  row[1] = find(2);
+  f32x4 acc[RT][4];
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) acc[rt][t] = f32x4{};
+#pragma unroll
+    for (int s = 0; s < NG; ++s)
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
+        acc[rt][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(lds.k[0][(t * NG + s) * 64 + lane], qf[rt][s], acc[rt][t],
+                                                            0, 0, 0);
+  }
 #pragma unroll
   for (int c = 0; c < 2; ++c) make_v(0, c);
-  uint64_t broken[4];
+  wait_loads();
+  codes = fresh;
+  load_k(row[1]);
 #pragma unroll
-  for (int t = 0; t < 4; ++t) broken[t] = lds.broken[0][t];
-  there[1] = start(1);
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  stage_params(1, there[1]);
+  for (int s = 0; s < NG; ++s) make_k(1, s);
+  stage_params(1, row[0]);
+  wait_loads();
   codes = fresh;
   __syncthreads();
 
   for (int n = 0; n < count; ++n) {
     const int key0 = (first + n) * kTile;
-    there[2] = start(n + 2);
-    uint64_t broken_next[4];
+    // in flight: K's tile n + 3, V's tile n + 2
+    row[2] = find(n + 3);
+    load_v(n + 2, row[1]);
+    load_k(row[2]);
+    const u32x4 flags = *reinterpret_cast<const u32x4*>(lds.flags[n & 3]);
+    const uint32_t all = __builtin_amdgcn_readfirstlane(flags[0] & flags[1] & flags[2] & flags[3]);
+    const uint32_t some = __builtin_amdgcn_readfirstlane(flags[0] | flags[1] | flags[2] | flags[3]);
+    const f16x8* const kf = lds.k[(n + 1) & 1] + lane;
+    const f16x8* const vf = lds.v[n & 1] + lane;
+    if (key0 + kTile > all_see || (all & 1) == 0) {
+      const uint32_t there = (flags[0] & 1) | (flags[1] & 1) << 1 | (flags[2] & 1) << 2 | (flags[3] & 1) << 3;
 #pragma unroll
-    for (int t = 0; t < 4; ++t) broken_next[t] = lds.broken[(n + 1) & 1][t];
-    if (rows_there && key0 < some_see) {
-      // The operands of a step are read one step ahead, and the next tile's are made in the shadow of
-      // the products (the barriers keep the compiler from moving the reads back to their uses).
-      const f16x8* const kf = lds.k[n & 1] + lane;
-      const f16x8* const vf = lds.v[n & 1] + lane;
-      f32x4 acc[RT][4];
-      f16x8 x[2][4];
+      for (int rt = 0; rt < RT; ++rt) mask_tile(acc[rt], limit[rt], there, key0 + 4 * g);
+    }
+    // ---- scores of tile n + 1 beside the softmax of tile n ----
+    f32x4 ahead[RT][4];
+    f16x8 x[2][4], pf[RT][2];
+    auto read_keys = [&](int s) {
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        x[0][t] = kf[t * NG * 64];
+      for (int t = 0; t < 4; ++t) x[s & 1][t] = kf[(t * NG + s) * 64];
+    };
+    auto scores = [&](int s) {
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) acc[rt][t] = f32x4{};
-      }
+      for (int t = 0; t < 4; ++t)
 #pragma unroll
-      for (int s = 0; s < NG; ++s) {
-        __builtin_amdgcn_sched_barrier(0);
+        for (int rt = 0; rt < RT; ++rt)
+          ahead[rt][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[s & 1][t], qf[rt][s], s == 0 ? f32x4{} : ahead[rt][t],
+                                                                0, 0, 0);
+    };
+    read_keys(0);
+    float hi[RT];
 #pragma unroll
-        for (int t = 0; t < 4; ++t) x[(s + 1) & 1][t] = s + 1 < NG ? kf[(t * NG + s + 1) * 64] : vf[t * 64];
-        __builtin_amdgcn_sched_barrier(0);
+    for (int s = 0; s < (NG + 1) / 2; ++s) {
+      if (s + 1 < NG) read_keys(s + 1);
+      scores(s);
+    }
 #pragma unroll
-        for (int t = 0; t < 4; ++t)
+    for (int rt = 0; rt < RT; ++rt) hi[rt] = tile_max(acc[rt], scale[rt]);
+    interleave<4 * RT * ((NG + 1) / 2), 3, 0>();
 #pragma unroll
-          for (int rt = 0; rt < RT; ++rt)
-            acc[rt][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[s & 1][t], qf[rt][s], acc[rt][t], 0, 0, 0);
-        make_k(n + 1, s);
-      }
+    for (int rt = 0; rt < RT; ++rt) raise_max(hi[rt], top[rt], sum[rt], o[rt]);
+#pragma unroll
+    for (int s = (NG + 1) / 2; s < NG; ++s) {
+      if (s + 1 < NG) read_keys(s + 1);
+      scores(s);
+    }
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) tile_weights(acc[rt], scale[rt], top[rt], pf[rt]);
+    interleave<4 * RT * (NG / 2), 3, 2>();
+    // ---- values of tile n beside the conversion of what comes next ----
+    __builtin_amdgcn_sched_barrier(0);
+    auto read_values = [&](int c) {  // operands 4 c .. 4 c + 3: channels 2 c and 2 c + 1 of 16, two words each
+#pragma unroll
+      for (int t = 0; t < 4; ++t) x[c & 1][t] = vf[(4 * c + t) * 64];
+    };
+    read_values(0);
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) sum[rt] = add_weights(pf[rt], sum[rt]);
+#pragma unroll
+    for (int c = 0; c < NG; ++c) {
+      if (c + 1 < NG) read_values(c + 1);
+      i32x2 words;
+      ValueParams params;
+      if (NG == 4 && c < 2) params = read_v(n + 1, c, words);
       __builtin_amdgcn_sched_barrier(0);
-      const bool masked = key0 + kTile > all_see || there[0] != 15u;
-      f16x8 pf[RT][2];
-      softmax_tile(acc, o, top, sum, scale, limit, masked, there[0], key0 + 4 * g, pf);
-      // V's operands 4 c .. 4 c + 3 are the channels 2 c and 2 c + 1 of 16, two words each
 #pragma unroll
-      for (int c = 0; c < NG; ++c) {
-        const int at = (NG + c) & 1;
-        __builtin_amdgcn_sched_barrier(0);
-        if (c + 1 < NG) {
+      for (int t = 0; t < 4; ++t)
 #pragma unroll
-          for (int t = 0; t < 4; ++t) x[at ^ 1][t] = vf[(4 * (c + 1) + t) * 64];
-        }
-        i32x2 words;
-        ValueParams params;
-        if (NG == 4 && c < 2) params = read_v(n + 1, c, words);
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int t = 0; t < 4; ++t)
-#pragma unroll
-          for (int rt = 0; rt < RT; ++rt)
-            o[rt][2 * c + (t >> 1)] =
-                __builtin_amdgcn_mfma_f32_16x16x32_f16(x[at][t], pf[rt][t & 1], o[rt][2 * c + (t >> 1)], 0, 0, 0);
-        if (NG == 4 && c < 2) write_v(n + 1, c, words, params);
+        for (int rt = 0; rt < RT; ++rt)
+          o[rt][2 * c + (t >> 1)] =
+              __builtin_amdgcn_mfma_f32_16x16x32_f16(x[c & 1][t], pf[rt][t & 1], o[rt][2 * c + (t >> 1)], 0, 0, 0);
+      if (NG == 4 && c < 2) write_v(n + 1, c, words, params);
+      if (NG < 4 || c >= 2) {
+        make_k(n + 2, NG < 4 ? c : 2 * (c - 2));
+        if (NG == 4) make_k(n + 2, 2 * (c - 2) + 1);
       }
-      if (NG < 4) {
-#pragma unroll
-        for (int c = 0; c < 2; ++c) make_v(n + 1, c);
-      }
-      if ((broken[0] | broken[1] | broken[2] | broken[3]) != 0) poison_rows<NG>(o, broken, limit, key0);
-    } else {
-#pragma unroll
-      for (int s = 0; s < NG; ++s) make_k(n + 1, s);
+      interleave<4 * RT, 4, 0>();
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if (NG < 4) {
 #pragma unroll
       for (int c = 0; c < 2; ++c) make_v(n + 1, c);
     }
-    // tile n + 2 has arrived; its parameters take the place of tile n's, whose operands all waves have made
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    stage_params(n + 2, there[2]);
+    if ((some & 2) != 0) {
+      const uint64_t broken[4] = {lds.broken[n & 3][0], lds.broken[n & 3][1], lds.broken[n & 3][2], lds.broken[n & 3][3]};
+      poison_rows<NG>(o, broken, limit, key0);
+    }
+    // V's tile n + 2 has arrived; its parameters take the place of tile n's, whose operands all waves have made
+    wait_loads();
+    stage_params(n + 2, row[1]);
     codes = fresh;
-    there[0] = there[1];
-    there[1] = there[2];
+    row[1] = row[2];
 #pragma unroll
-    for (int t = 0; t < 4; ++t) broken[t] = broken_next[t];
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) acc[rt][t] = ahead[rt][t];
     __syncthreads();
   }
 
@@ -836,7 +891,7 @@ __global__ void __launch_bounds__(kWaves * 64, 2) kv4_chunk_kernel(const Kv4Args
   const int64_t item = ((int64_t)(it.b * a.hk + it.h) * a.row_blocks + rb) * a.splits + split;
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
-    const float all = lanes16_sum(sum[rt]);
+    const float all = sum[rt][0];
     const int row = row0 + 16 * rt + i, token = fast_div(row, a.by_group), head = row - token * a.group;
     if (row >= it.rows) continue;
     const int64_t part = item * kRows + wave * 16 * RT + 16 * rt + i;
