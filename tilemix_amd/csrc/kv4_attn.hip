@@ -787,27 +787,30 @@ __global__ void __launch_bounds__(kWaves * 64, 2) kv4_chunk_kernel(const Kv4Args
 
   for (int n = 0; n < count; ++n) {
     const int key0 = (first + n) * kTile;
+    const f16x8* const kf = lds.k[(n + 1) & 1] + lane;
+    const f16x8* const vf = lds.v[n & 1] + lane;
+    f16x8 x[2][4], pf[RT][2];
+    auto read_keys = [&](int s) {
+#pragma unroll
+      for (int t = 0; t < 4; ++t) x[s & 1][t] = kf[(t * NG + s) * 64];
+    };
+    read_keys(0);
+    const u32x4 flags = *reinterpret_cast<const u32x4*>(lds.flags[n & 3]);
+    __builtin_amdgcn_sched_barrier(0);
     // in flight: K's tile n + 3, V's tile n + 2
     row[2] = find(n + 3);
     load_v(n + 2, row[1]);
     load_k(row[2]);
-    const u32x4 flags = *reinterpret_cast<const u32x4*>(lds.flags[n & 3]);
     const uint32_t all = __builtin_amdgcn_readfirstlane(flags[0] & flags[1] & flags[2] & flags[3]);
     const uint32_t some = __builtin_amdgcn_readfirstlane(flags[0] | flags[1] | flags[2] | flags[3]);
-    const f16x8* const kf = lds.k[(n + 1) & 1] + lane;
-    const f16x8* const vf = lds.v[n & 1] + lane;
     if (key0 + kTile > all_see || (all & 1) == 0) {
       const uint32_t there = (flags[0] & 1) | (flags[1] & 1) << 1 | (flags[2] & 1) << 2 | (flags[3] & 1) << 3;
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt) mask_tile(acc[rt], limit[rt], there, key0 + 4 * g);
     }
     // ---- scores of tile n + 1 beside the softmax of tile n ----
+    __builtin_amdgcn_s_setprio(1);
     f32x4 ahead[RT][4];
-    f16x8 x[2][4], pf[RT][2];
-    auto read_keys = [&](int s) {
-#pragma unroll
-      for (int t = 0; t < 4; ++t) x[s & 1][t] = kf[(t * NG + s) * 64];
-    };
     auto scores = [&](int s) {
 #pragma unroll
       for (int t = 0; t < 4; ++t)
@@ -816,7 +819,6 @@ __global__ void __launch_bounds__(kWaves * 64, 2) kv4_chunk_kernel(const Kv4Args
           ahead[rt][t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(x[s & 1][t], qf[rt][s], s == 0 ? f32x4{} : ahead[rt][t],
                                                                 0, 0, 0);
     };
-    read_keys(0);
     float hi[RT];
 #pragma unroll
     for (int s = 0; s < (NG + 1) / 2; ++s) {
@@ -837,6 +839,7 @@ __global__ void __launch_bounds__(kWaves * 64, 2) kv4_chunk_kernel(const Kv4Args
     for (int rt = 0; rt < RT; ++rt) tile_weights(acc[rt], scale[rt], top[rt], pf[rt]);
     interleave<4 * RT * (NG / 2), 3, 2>();
     // ---- values of tile n beside the conversion of what comes next ----
+    __builtin_amdgcn_s_setprio(0);
     __builtin_amdgcn_sched_barrier(0);
     auto read_values = [&](int c) {  // operands 4 c .. 4 c + 3: channels 2 c and 2 c + 1 of 16, two words each
 #pragma unroll
@@ -853,11 +856,13 @@ __global__ void __launch_bounds__(kWaves * 64, 2) kv4_chunk_kernel(const Kv4Args
       if (NG == 4 && c < 2) params = read_v(n + 1, c, words);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int t = 0; t < 4; ++t)
+      for (int w = 0; w < 2; ++w)
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
-          o[rt][2 * c + (t >> 1)] =
-              __builtin_amdgcn_mfma_f32_16x16x32_f16(x[c & 1][t], pf[rt][t & 1], o[rt][2 * c + (t >> 1)], 0, 0, 0);
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt)
+            o[rt][2 * c + k] =
+                __builtin_amdgcn_mfma_f32_16x16x32_f16(x[c & 1][2 * k + w], pf[rt][w], o[rt][2 * c + k], 0, 0, 0);
       if (NG == 4 && c < 2) write_v(n + 1, c, words, params);
       if (NG < 4 || c >= 2) {
         make_k(n + 2, NG < 4 ? c : 2 * (c - 2));
@@ -982,7 +987,7 @@ bool make_plan(const char* what, const tilemix_kv4_attn_params& p, Plan& plan) {
   const int64_t items = std::max<int64_t>(blocks * p.heads_k * p.batch, 1);
   const int64_t wanted = std::max<int64_t>(1, (int64_t)(plan.block_rows < kChunkRows ? 1024 : 512) / items);
   int64_t split_tiles = (tiles + wanted - 1) / wanted;
-  split_tiles = (split_tiles + kWaves - 1) / kWaves * kWaves;
+  if (plan.block_rows < kChunkRows) split_tiles = (split_tiles + kWaves - 1) / kWaves * kWaves;
   const int64_t splits = (tiles + split_tiles - 1) / split_tiles;
   const int64_t grid = blocks * splits;
   if (rows > INT32_MAX / 2 || grid > (plan.block_rows < kChunkRows ? (1 << 24) - 1 : 65535) || items * splits > INT32_MAX / 64) {
