@@ -152,9 +152,19 @@ __device__ __forceinline__ void copy16(const uint32_t* base, uint32_t offset, ui
       : "memory");
 }
 
-// The keys of one wave: tiles first + wave, + kWaves, ..  Tile n of them has its blocks' rows of the pool
-// in the lanes 4 (n % 16) .. + 3 of `rows` (-1: no page, or behind `end`), from one load of the block table for
-// every 16 tiles, made 16 tiles ahead.
+// A table entry for a key, within the table's columns whatever the key (the loads of the sequence's bounds, which
+// say what the entry is worth, are on their way at the same time).
+__device__ __forceinline__ int table_entry(const Kv4Args& a, const int32_t* table, int key) {
+  return a.columns > 0 ? table[min(fast_div(key, a.by_page), a.columns - 1)] : -1;
+}
+// The row of the pool of a block's first key: -1 where there is no page, or the block is at or behind `end`.
+__device__ __forceinline__ int block_row(const Kv4Args& a, int id, int h, int key, int end) {
+  const int column = fast_div(key, a.by_page);
+  return key < end && id >= 0 && id < a.pages ? (id * a.hk + h) * a.by_page.d + (key - column * a.by_page.d) : -1;
+}
+
+// The keys of one wave: tiles first + wave, + kWaves, ..  Tile n of them has its blocks' rows in the
+// lanes 4 (n % 16) .. + 3 of `rows`, from one load of the block table for every 16 tiles, made 16 tiles ahead.
 struct Kv4Walk {
   const int32_t* table;
   int key0, end;  // first key of the wave; no block at or behind `end`
@@ -164,14 +174,8 @@ struct Kv4Walk {
     const int lane = threadIdx.x & 63;
     return key0 + (n + (lane >> 2)) * (kWaves * kTile) + 16 * (lane & 3);
   }
-  __device__ __forceinline__ int fetch(const Kv4Args& a, int n) const {
-    const int k = key(n);
-    return k < end ? table[fast_div(k, a.by_page)] : -1;
-  }
-  __device__ __forceinline__ void use(const Kv4Args& a, int h, int n) {
-    const int k = key(n), column = fast_div(k, a.by_page);
-    rows = ids >= 0 && ids < a.pages ? (ids * a.hk + h) * a.by_page.d + (k - column * a.by_page.d) : -1;
-  }
+  __device__ __forceinline__ void fetch(const Kv4Args& a, int n) { ids = table_entry(a, table, key(n)); }
+  __device__ __forceinline__ void use(const Kv4Args& a, int h, int n) { rows = block_row(a, ids, h, key(n), end); }
 };
 
 // Starts the loads of tile n (V codes into LDS); there: which of its blocks have a page.  A block without
@@ -208,7 +212,7 @@ __device__ __forceinline__ uint32_t load_tile(Kv4Tile<NG>& x, const Kv4Args& a, 
 }
 
 // Elements c .. c + n - 1 (n <= 8) of a query row, zeros behind them.
-__device__ __forceinline__ f32x8 load_query(const uint16_t* row, int c, int n, bool vec, bool bf) {
+__device__ __forceinline__ u32x4 load_query(const uint16_t* row, int c, int n, bool vec) {
   u32x4 w;
   if (vec && n == 8) {
     w = *reinterpret_cast<const u32x4*>(row + c);
@@ -219,15 +223,7 @@ __device__ __forceinline__ f32x8 load_query(const uint16_t* row, int c, int n, b
       w[e] = (2 * e < n ? lo : 0u) | (2 * e + 1 < n ? hi << 16 : 0u);
     }
   }
-  f32x8 x;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    const uint32_t pair = w[e];  // (a bit cast of a vector's element would take the first one)
-    const f16x2 h = __builtin_bit_cast(f16x2, pair);
-    x[2 * e] = bf ? __uint_as_float(pair << 16) : (float)h[0];
-    x[2 * e + 1] = bf ? __uint_as_float(pair & 0xffff0000u) : (float)h[1];
-  }
-  return x;
+  return w;
 }
 
 // Rounds four channels to the output's type and writes those below d.
@@ -245,31 +241,47 @@ __device__ __forceinline__ void store_out(void* out, int64_t at, const f32x4& r,
   }
 }
 
-// The queries of rows row0 + 16 rt + i as B operand of QK, the factor of their products and the keys they see.
+// The queries of rows row0 + 16 rt + i, channels 8 (NG g + s) .. + 7, as they lie in memory.  A row that is not
+// there reads the block's first one and becomes zeros.
 template <int NG, int RT>
-__device__ __forceinline__ void load_queries(const Kv4Args& a, const Kv4Item& it, int row0, f16x8 (&qf)[RT][NG],
-                                             float (&scale)[RT], int (&limit)[RT]) {
+__device__ __forceinline__ void load_queries(const Kv4Args& a, const Kv4Item& it, int row0, u32x4 (&raw)[RT][NG]) {
   const int lane = threadIdx.x & 63, i = lane & 15, g = lane >> 4;
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
-    const int row = row0 + 16 * rt + i, token = fast_div(row, a.by_group), head = row - token * a.group;
-    const bool there = row < it.rows;
-    limit[rt] = a.causal ? it.limit0 + token : it.len;
+    const bool there = row0 + 16 * rt + i < it.rows;
+    const int row = there ? row0 + 16 * rt + i : row0, token = fast_div(row, a.by_group), head = row - token * a.group;
+    const uint16_t* const from =
+        static_cast<const uint16_t*>(a.q) + (it.start + token) * a.sq_t + (it.h * a.group + head) * a.sq_h;
+#pragma unroll
+    for (int s = 0; s < NG; ++s) {
+      const int c = 8 * (NG * g + s);
+      raw[rt][s] = load_query(from, c, there ? min(8, a.d - c) : 0, a.q_vec);
+    }
+  }
+}
+
+// The same as B operand of QK, the factor of their products and the keys that the rows see.
+template <int NG, int RT>
+__device__ __forceinline__ void use_queries(const Kv4Args& a, const Kv4Item& it, int row0, const u32x4 (&raw)[RT][NG],
+                                            f16x8 (&qf)[RT][NG], float (&scale)[RT], int (&limit)[RT]) {
+  const int i = threadIdx.x & 15;
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    limit[rt] = a.causal ? it.limit0 + fast_div(row0 + 16 * rt + i, a.by_group) : it.len;
     // A negative scale is the queries' sign; none is a product that leaves the maximum at zero.
     scale[rt] = fmaxf(fabsf(a.scale), 1e-37f);
-    // a row that is not there reads the block's first one and becomes zeros
-    const uint16_t* const from =
-        static_cast<const uint16_t*>(a.q) + (it.start + (there ? token : fast_div(row0, a.by_group))) * a.sq_t +
-        (it.h * a.group + (there ? head : row0 - fast_div(row0, a.by_group) * a.group)) * a.sq_h;
     f32x8 x[NG];
     float top = 0.0f;
 #pragma unroll
-    for (int s = 0; s < NG; ++s) {
-      const int c = 8 * (NG * g + s), n = there ? min(8, a.d - c) : 0;
-      x[s] = load_query(from, c, n, a.q_vec, a.bf);
+    for (int s = 0; s < NG; ++s)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[s][e]));
-    }
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t pair = raw[rt][s][e];  // (a bit cast of a vector's element would take the first one)
+        const f16x2 h = __builtin_bit_cast(f16x2, pair);
+        x[s][2 * e] = a.bf ? __uint_as_float(pair << 16) : (float)h[0];
+        x[s][2 * e + 1] = a.bf ? __uint_as_float(pair & 0xffff0000u) : (float)h[1];
+        top = fmaxf(top, fmaxf(fabsf(x[s][2 * e]), fabsf(x[s][2 * e + 1])));
+      }
     // bf16 queries are held as fp16 times a power of two of their row: exact but for elements below
     // 2^-14 of the row's largest, which lose no more than 2^-25 of that one.
     if (a.bf) {
@@ -414,24 +426,38 @@ __global__ void __launch_bounds__(kWaves * 64, RT == 1 ? 3 : 2) kv4_attn_kernel(
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15,
             g = lane >> 4;
   const int rb = fast_div(blockIdx.x, a.by_splits), split = blockIdx.x - rb * a.splits;
+  const int first = split * a.split_tiles;
   const Kv4Item it = kv4_item(a, blockIdx.z, blockIdx.y, rb, 16 * RT);
   const int row0 = rb * 16 * RT;
   if (row0 >= it.rows) return;
   const int tiles = it.kmax <= 0 ? 0 : (it.kmax + kTile - 1) / kTile;
-  const int first = split * a.split_tiles, last = min(tiles, first + a.split_tiles);
+  const int last = min(tiles, first + a.split_tiles);
   if (first >= last && split > 0) return;
 
-  // ---- the first keys' places are on their way while the queries come ----
+  // the first keys' places are on their way while the queries come
   Kv4Walk walk;
   walk.table = a.table + it.b * a.s_table;
   walk.key0 = (first + wave) * kTile;
   walk.end = min(it.kmax, last * kTile);
-  walk.ids = walk.fetch(a, 0);
-
+  walk.fetch(a, 0);
   f16x8 qf[RT][NG];
   float scale[RT];
   int limit[RT];
-  load_queries(a, it, row0, qf, scale, limit);
+  {
+    u32x4 raw[RT][NG];
+    load_queries(a, it, row0, raw);
+    use_queries(a, it, row0, raw, qf, scale, limit);
+  }
+
+  unsigned char* const lds_v = smem + wave * kWaveLds<NG>;
+  f16* const lds_s = reinterpret_cast<f16*>(lds_v + 2 * 4 * kBlockLds);
+  f16* const lds_m = lds_s + NG * 64;
+  const uint32_t v_addr = lds_addr(lds_v);
+  Tile x;
+  walk.use(a, it.h, 0);
+  walk.fetch(a, 16);
+  uint32_t there = load_tile(x, a, walk, 0, v_addr);
+
   f32x4 o[RT][kCT];
   float top[RT];
   f32x4 sum[RT];  // four times the same
@@ -443,19 +469,11 @@ __global__ void __launch_bounds__(kWaves * 64, RT == 1 ? 3 : 2) kv4_attn_kernel(
     for (int ct = 0; ct < kCT; ++ct) o[rt][ct] = f32x4{};
   }
 
-  unsigned char* const lds_v = smem + wave * kWaveLds<NG>;
-  f16* const lds_s = reinterpret_cast<f16*>(lds_v + 2 * 4 * kBlockLds);
-  f16* const lds_m = lds_s + NG * 64;
-  const uint32_t v_addr = lds_addr(lds_v);
   const int all_see = it.limit0 + (a.causal ? fast_div(row0, a.by_group) : 0);  // keys that every row sees
   // V rows that the lane points at in a transposed read, in LDS
   const int v_at = (i >> 2) * kBlockLds + (4 * g + (i & 3)) * 16;
   const int p_at = 16 * (i >> 2) + 2 * (i & 3);  // of key i of a block in the pairs' order, see below
 
-  Tile x;
-  walk.use(a, it.h, 0);
-  walk.ids = walk.fetch(a, 16);
-  uint32_t there = load_tile(x, a, walk, 0, v_addr);
   int n = 0;
   for (int tile = first + wave; tile < last; tile += kWaves, ++n) {
     const int key0 = tile * kTile;
@@ -510,7 +528,7 @@ __global__ void __launch_bounds__(kWaves * 64, RT == 1 ? 3 : 2) kv4_attn_kernel(
     const uint32_t here = there;
     if (((n + 1) & 15) == 0) {
       walk.use(a, it.h, n + 1);
-      walk.ids = walk.fetch(a, n + 17);
+      walk.fetch(a, n + 17);
     }
     there = load_tile(x, a, walk, n + 1, v_addr + ((n + 1) & 1) * 4 * kBlockLds);
     __builtin_amdgcn_sched_barrier(0);
@@ -636,40 +654,19 @@ __global__ void __launch_bounds__(kWaves * 64, 2) kv4_chunk_kernel(const Kv4Args
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15,
             g = lane >> 4;
   const int rb = fast_div(blockIdx.y, a.by_splits), split = blockIdx.y - rb * a.splits;
+  const int first = split * a.split_tiles;
+  // The rows of the pool of block `wave` of the tiles first + 64 c .. + 63, one in each lane (-1: no page).
+  const int32_t* const table = a.table + blockIdx.z * a.s_table;
+  auto key_of = [&](int n) { return (first + n + lane) * kTile + 16 * wave; };
+  int ids = table_entry(a, table, key_of(0)), rows = -1;
   const Kv4Item it = kv4_item(a, blockIdx.z, blockIdx.x, rb, kRows);
   if (rb * kRows >= it.rows) return;
   const int tiles = it.kmax <= 0 ? 0 : (it.kmax + kTile - 1) / kTile;
-  const int first = split * a.split_tiles, last = min(tiles, first + a.split_tiles);
+  const int last = min(tiles, first + a.split_tiles);
   if (first >= last && split > 0) return;
   const int end = min(it.kmax, last * kTile);  // keys
 
-  // The rows of the pool of block `wave` of the tiles first + 64 c .. + 63, one in each lane (-1: no page).
-  const int32_t* const table = a.table + it.b * a.s_table;
-  auto fetch = [&](int n) {
-    const int key = (first + n + lane) * kTile + 16 * wave;
-    return key < end ? table[fast_div(key, a.by_page)] : -1;
-  };
-  int ids = fetch(0), rows = -1;
-
   const int row0 = rb * kRows + wave * 16 * RT;  // of the wave
-  f16x8 qf[RT][NG];
-  float scale[RT];
-  int limit[RT];
-  load_queries(a, it, min(row0, it.rows - 1), qf, scale, limit);
-  const bool rows_there = row0 < it.rows;
-  const int all_see = it.limit0 + (a.causal ? fast_div(row0, a.by_group) : 0);  // keys that all rows of the wave see
-
-  f32x4 o[RT][kCT];
-  float top[RT];
-  f32x4 sum[RT];  // four times the same
-#pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-    top[rt] = kNoKey;
-    sum[rt] = f32x4{};
-#pragma unroll
-    for (int ct = 0; ct < kCT; ++ct) o[rt][ct] = f32x4{};
-  }
-
   // ---- loads ----
   const int gc = g < NG ? g : NG - 1;
   const uint32_t words_at = i * (4 * NG) + NG * g, chunk_at = 16 * (i * NG + gc), group_at = i * NG + gc;
@@ -680,9 +677,8 @@ __global__ void __launch_bounds__(kWaves * 64, 2) kv4_chunk_kernel(const Kv4Args
   uint32_t vp;
   auto find = [&](int n) {  // the row of the wave's block of tile n
     if ((n & 63) == 0) {
-      const int key = (first + n + lane) * kTile + 16 * wave, column = fast_div(key, a.by_page);
-      rows = ids >= 0 && ids < a.pages ? (ids * a.hk + it.h) * a.by_page.d + (key - column * a.by_page.d) : -1;
-      ids = fetch(n + 64);
+      rows = block_row(a, ids, it.h, key_of(n), end);
+      ids = table_entry(a, table, key_of(n + 64));
     }
     return __builtin_amdgcn_readlane(rows, n & 63);
   };
@@ -744,23 +740,56 @@ __global__ void __launch_bounds__(kWaves * 64, 2) kv4_chunk_kernel(const Kv4Args
     }
   };
 
+  u32x4 raw[RT][NG];
+  load_queries(a, it, min(row0, it.rows - 1), raw);
   // ---- before tile 0: its scores, its values, K's tile 1, the codes of K's tile 2 and V's tile 1 ----
   const int count = last - first;
   int row[3];  // of the wave's block of tiles n + 1 .. n + 3
   auto wait_loads = [] { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); };
-  row[1] = find(0);
-  load_k(row[1]);
-  load_v(0, row[1]);
-  row[0] = find(1);
-  wait_loads();
-  stage_params(0, row[1]);
-  codes = fresh;
-  load_k(row[0]);
 #pragma unroll
-  for (int s = 0; s < NG; ++s) make_k(0, s);
+  for (int k = 0; k < 3; ++k) row[k] = find(k);
+  KeyCodes ahead_codes[3];
+#pragma unroll
+  for (int k = 0; k < 3; ++k) {
+    load_k(row[k]);
+    ahead_codes[k] = fresh;
+  }
+  load_v(0, row[0]);
+  const uint32_t vp0 = vp;
+  load_v(1, row[1]);
+  const uint32_t vp1 = vp;
+  f16x8 qf[RT][NG];
+  float scale[RT];
+  int limit[RT];
+  use_queries(a, it, min(row0, it.rows - 1), raw, qf, scale, limit);
+  const bool rows_there = row0 < it.rows;
+  const int all_see = it.limit0 + (a.causal ? fast_div(row0, a.by_group) : 0);  // keys that all rows of the wave see
+
+  f32x4 o[RT][kCT];
+  float top[RT];
+  f32x4 sum[RT];  // four times the same
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    top[rt] = kNoKey;
+    sum[rt] = f32x4{};
+#pragma unroll
+    for (int ct = 0; ct < kCT; ++ct) o[rt][ct] = f32x4{};
+  }
+
+  wait_loads();
+  vp = vp0;
+  stage_params(0, row[0]);
+  vp = vp1;
+  stage_params(1, row[1]);
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    codes = ahead_codes[k];
+#pragma unroll
+    for (int s = 0; s < NG; ++s) make_k(k, s);
+  }
+  codes = ahead_codes[2];
+  row[1] = row[2];
   __syncthreads();
-  load_v(1, row[0]);
-  row[1] = find(2);
   f32x4 acc[RT][4];
 #pragma unroll
   for (int t = 0; t < 4; ++t) {
@@ -775,14 +804,6 @@ __global__ void __launch_bounds__(kWaves * 64, 2) kv4_chunk_kernel(const Kv4Args
   }
 #pragma unroll
   for (int c = 0; c < 2; ++c) make_v(0, c);
-  wait_loads();
-  codes = fresh;
-  load_k(row[1]);
-#pragma unroll
-  for (int s = 0; s < NG; ++s) make_k(1, s);
-  stage_params(1, row[0]);
-  wait_loads();
-  codes = fresh;
   __syncthreads();
 
   for (int n = 0; n < count; ++n) {
