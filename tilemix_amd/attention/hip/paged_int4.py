@@ -41,12 +41,17 @@ class PagedInt4Cache:
     low half of byte j; width is head_dim rounded up to 32) and ``params`` fp16
     [pages, heads, page_size, width / 32, 2] (scale, minimum), contiguous.  page_size is a multiple of 16."""
 
-    __slots__ = ("k_codes", "k_params", "v_codes", "v_params", "head_dim")
+    __slots__ = ("_args",)
 
     def __init__(self, k_codes: Tensor, k_params: Tensor, v_codes: Tensor, v_params: Tensor, head_dim: int):
         _native.host().kv4_check(k_codes, k_params, v_codes, v_params, head_dim)
-        self.k_codes, self.k_params, self.v_codes, self.v_params = k_codes, k_params, v_codes, v_params
-        self.head_dim = head_dim
+        self._args = (k_codes, k_params, v_codes, v_params, head_dim)
+
+    k_codes = property(lambda self: self._args[0])
+    k_params = property(lambda self: self._args[1])
+    v_codes = property(lambda self: self._args[2])
+    v_params = property(lambda self: self._args[3])
+    head_dim = property(lambda self: self._args[4])
 
     @classmethod
     def empty(cls, pages: int, heads: int, head_dim: int, page_size: int = 64, device="cuda") -> "PagedInt4Cache":
@@ -68,10 +73,6 @@ class PagedInt4Cache:
     def page_size(self) -> int:
         return self.k_codes.shape[2]
 
-    @property
-    def _args(self):
-        return self.k_codes, self.k_params, self.v_codes, self.v_params, self.head_dim
-
 
 class SlotPlan(NamedTuple):
     """Where the new tokens of a step go (``PageTables.extend``)."""
@@ -89,12 +90,16 @@ class PageTables:
     in place, in the order of the stream they run on: calls on several streams have to be ordered by
     the caller.  One ``PageTables`` serves the caches of all layers."""
 
-    __slots__ = ("block_table", "seq_lens", "free_pages", "free_count", "page_size", "_ticket")
+    __slots__ = ("_args", "page_size")
 
     def __init__(self, block_table: Tensor, seq_lens: Tensor, free_pages: Tensor, free_count: Tensor, page_size: int):
-        self.block_table, self.seq_lens = block_table, seq_lens
-        self.free_pages, self.free_count, self.page_size = free_pages, free_count, page_size
-        self._ticket = torch.zeros(1, dtype=torch.int32, device=block_table.device)
+        ticket = torch.zeros(1, dtype=torch.int32, device=block_table.device)
+        self._args, self.page_size = (block_table, seq_lens, free_pages, free_count, ticket), page_size
+
+    block_table = property(lambda self: self._args[0])
+    seq_lens = property(lambda self: self._args[1])
+    free_pages = property(lambda self: self._args[2])
+    free_count = property(lambda self: self._args[3])
 
     @classmethod
     def empty(cls, pages: int, sequences: int, columns: int, page_size: int = 64, device="cuda") -> "PageTables":
@@ -103,10 +108,6 @@ class PageTables:
                    torch.zeros(sequences, dtype=torch.int32, device=device),
                    torch.arange(pages - 1, -1, -1, dtype=torch.int32, device=device),
                    torch.full((1,), pages, dtype=torch.int32, device=device), page_size)
-
-    @property
-    def _args(self):
-        return self.block_table, self.seq_lens, self.free_pages, self.free_count, self._ticket
 
     def extend(self, new_lens: Tensor, num_tokens: int) -> SlotPlan:
         """Give sequence b ``new_lens[b]`` (int32) more tokens; ``num_tokens``: entries of the plan, at

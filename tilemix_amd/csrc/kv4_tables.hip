@@ -2,8 +2,8 @@
 // sequences of a step, and pages back, without a word to the host.
 //
 // Both calls are bound by the launch and by a chain of dependent loads, not by bytes: every
-// workgroup sums the whole batch's lengths for itself (two prefix sums over at most 4096 sequences,
-// kept in LDS) and then serves its share of the tokens or pages by a search in them, which is
+// workgroup sums the whole batch's lengths for itself (prefix sums over at most 4096 sequences, kept
+// in LDS) and then serves its share of the tokens or pages by a search in them, which is
 // one launch.  The values that other workgroups read (seq_lens, free_count) are written by
 // the last one to have read them, which a ticket finds.
 #include "kv4_common.h"
@@ -16,6 +16,7 @@ namespace {
 
 constexpr int kMaxBatch = 4096;
 constexpr int kThreads = 256;
+constexpr int kTokens = 4;  // consecutive ones that a thread of kv4_extend_kernel serves
 
 struct TablesArgs {
   int32_t* table;
@@ -33,26 +34,35 @@ struct TablesArgs {
   FastDiv by_page;
 };
 
-// Sum of x over the workgroup's threads before this one; total: over all of them.
-__device__ __forceinline__ int64_t scan(int64_t x, int64_t* wave_sums, int64_t& total) {
+// x + the values of the lanes before it in the wave (saturating, so that sums past 32 bits stay past every bound).
+// Shifts within 16 lanes, then the last lane of a row to the rows behind it.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t add_shifted(uint32_t x) {
+  return __builtin_elementwise_add_sat(
+      x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xf, false));
+}
+__device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
+  x = add_shifted<0x111, 0xf>(x);
+  x = add_shifted<0x112, 0xf>(x);
+  x = add_shifted<0x114, 0xf>(x);
+  x = add_shifted<0x118, 0xf>(x);
+  x = add_shifted<0x142, 0xa>(x);
+  x = add_shifted<0x143, 0xc>(x);
+  return x;
+}
+
+// The sum over the workgroup's threads before this one; `sums`: a place of its own for every scan of a kernel.
+__device__ __forceinline__ uint32_t scan_before(uint32_t x, uint32_t* sums) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int64_t sum = x;
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const int64_t other = __shfl_up(sum, off, 64);
-    if (lane >= off) sum += other;
-  }
-  __syncthreads();  // the sums of the scan before are read
-  if (lane == 63) wave_sums[wave] = sum;
+  const uint32_t sum = wave_scan(x);
+  if (lane == 63) sums[wave] = sum;
   __syncthreads();
-  int64_t before = 0;
-  total = 0;
+  uint32_t before = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)sum, 0x138, 0xf, 0xf, false);  // the lane before
+  if (lane == 0) before = 0;
 #pragma unroll
-  for (int i = 0; i < kThreads / 64; ++i) {
-    if (i < wave) before += wave_sums[i];
-    total += wave_sums[i];
-  }
-  return before + sum - x;
+  for (int i = 0; i < kThreads / 64 - 1; ++i)
+    if (i < wave) before = __builtin_elementwise_add_sat(before, sums[i]);
+  return before;
 }
 
 // The last entry i <= n - 1 of ascending first[] with first[i] <= x (first[0] <= x).
@@ -66,16 +76,14 @@ __device__ __forceinline__ int find(const int32_t* first, int n, int x) {
   return lo;
 }
 
-// True in all threads of the workgroup that comes here last; the others' loads are done by then.
+// True in all threads of the workgroup that comes here last: seq_lens, free_count and the new lengths have been
+// read by all then (their values are in LDS).  Nothing that the others wrote is read, so the count need not order it.
 __device__ __forceinline__ bool last_workgroup(const TablesArgs& a) {
   __shared__ int last;
-  __syncthreads();
+  if (gridDim.x == 1) return true;
   if (threadIdx.x == 0) {
-    last = 1;
-    if (gridDim.x > 1) {
-      last = __hip_atomic_fetch_add(a.ticket, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT) == (int)gridDim.x - 1;
-      if (last) __hip_atomic_store(a.ticket, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    }
+    last = __hip_atomic_fetch_add(a.ticket, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (int)gridDim.x - 1;
+    if (last) __hip_atomic_store(a.ticket, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
   __syncthreads();
   return last != 0;
@@ -88,112 +96,126 @@ __device__ __forceinline__ int clamp_int(int64_t x, int64_t lo, int64_t hi) {
 // LDS: cu [batch + 1], base [batch] (pages taken before; -1: nothing granted), old [batch] (tokens held)
 __global__ void __launch_bounds__(kThreads) kv4_extend_kernel(const TablesArgs a) {
   extern __shared__ int32_t lds[];
-  __shared__ int64_t wave_sums[kThreads / 64];
+  __shared__ uint32_t sums[2][kThreads / 64];
   int32_t* const cu = lds;
   int32_t* const base = cu + a.batch + 1;
   int32_t* const old = base + a.batch;
   const int page = a.by_page.d;
   const int64_t room = min((int64_t)a.columns * page, (int64_t)INT32_MAX - page);
   const int count = clamp_int(*a.count, 0, a.capacity);
-  int64_t tokens_before = 0, pages_before = 0, taken = 0;
-  for (int r0 = 0; r0 < a.batch; r0 += kThreads) {
-    const int r = r0 + threadIdx.x;
-    int64_t change = 0;
-    int held = 0;
-    if (r < a.batch) {
-      change = a.change[r];
-      held = clamp_int(a.lens[r], 0, room);
-    }
-    const bool wanted = r < a.batch && change >= 0;
-    if (change < 0) change = 0;
-    int64_t total;
-    const int64_t start = tokens_before + scan(change, wave_sums, total), end = start + change;
-    tokens_before += total;
-    const bool fits = wanted && end <= a.tokens && held + change <= room;
-    const int have = fast_div(held + page - 1, a.by_page);
-    const int needs = fits ? fast_div((int)(held + change) + page - 1, a.by_page) - have : 0;
-    const int64_t first = pages_before + scan(needs, wave_sums, total);
-    pages_before += total;
-    const bool ok = fits && (needs == 0 || first + needs <= count);
-    if (r < a.batch) {
-      cu[r] = clamp_int(start, 0, a.tokens);
-      base[r] = ok ? (needs == 0 ? 0 : (int)first) : -1;
-      old[r] = held;
-      if (r == a.batch - 1) cu[a.batch] = clamp_int(end, 0, a.tokens);
-      if (blockIdx.x == 0) {
-        a.granted[r] = ok;
-        a.cu[r] = clamp_int(start, 0, a.tokens);
-        if (r == a.batch - 1) a.cu[a.batch] = clamp_int(end, 0, a.tokens);
-      }
-    }
-    // what is granted ends where the needs first exceed the stack: the largest first + needs within it
-    int64_t got = ok && needs > 0 ? first + needs : 0;
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) got = max(got, (int64_t)__shfl_xor(got, off, 64));
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) wave_sums[threadIdx.x >> 6] = got;
-    __syncthreads();
-#pragma unroll
-    for (int i = 0; i < kThreads / 64; ++i) taken = max(taken, wave_sums[i]);
+  // Each thread has the same number of consecutive sequences.
+  const int each = (a.batch + kThreads - 1) / kThreads, r0 = threadIdx.x * each, r1 = min(r0 + each, a.batch);
+  uint32_t mine = 0;
+  for (int r = r0; r < r1; ++r) {
+    const int change = a.change[r];
+    old[r] = clamp_int(a.lens[r], 0, room);
+    base[r] = change;
+    mine = __builtin_elementwise_add_sat(mine, (uint32_t)max(change, 0));
+  }
+  const uint32_t tokens_before = scan_before(mine, sums[0]);
+  uint32_t at = tokens_before, pages = 0;
+  for (int r = r0; r < r1; ++r) {
+    const int change = base[r], held = old[r];
+    cu[r] = (int)min((int64_t)at, a.tokens);
+    at = __builtin_elementwise_add_sat(at, (uint32_t)max(change, 0));
+    const bool fits = change >= 0 && at <= (uint32_t)a.tokens && (int64_t)held + change <= room;
+    const int needs = fits ? fast_div(held + change + page - 1, a.by_page) - fast_div(held + page - 1, a.by_page) : -1;
+    base[r] = needs;
+    pages = __builtin_elementwise_add_sat(pages, (uint32_t)max(needs, 0));
+  }
+  if (r1 == a.batch && r0 < r1) cu[a.batch] = (int)min((int64_t)at, a.tokens);
+  uint32_t first = scan_before(pages, sums[1]);
+  for (int r = r0; r < r1; ++r) {
+    const int needs = base[r];
+    const uint32_t behind = __builtin_elementwise_add_sat(first, (uint32_t)max(needs, 0));
+    base[r] = needs < 0 || (needs > 0 && behind > (uint32_t)count) ? -1 : needs == 0 ? 0 : (int)first;
+    first = behind;
   }
   __syncthreads();
   const int end = cu[a.batch];
-  for (int64_t t = (int64_t)blockIdx.x * kThreads + threadIdx.x; t < a.tokens; t += (int64_t)gridDim.x * kThreads) {
-    int64_t slot = -1, position = 0;
-    if (t < end) {
-      const int r = find(cu, a.batch, (int)t);
-      if (base[r] >= 0) {
-        const int at = old[r] + (int)t - cu[r], column = fast_div(at, a.by_page);
-        const int have = fast_div(old[r] + page - 1, a.by_page), in_page = at - column * page;
-        int32_t* const entry = a.table + r * a.s_table + column;
-        int id;
-        if (column < have) {
-          id = *entry;
-        } else {
-          id = a.stack[count - 1 - (base[r] + column - have)];
-          if (in_page == 0) *entry = id;
-        }
-        position = at;
-        slot = id < 0 ? -1 : (int64_t)id * page + in_page;
-      }
+  // kTokens consecutive tokens a thread: one search for them, and their loads in flight together.
+  const int64_t step = (int64_t)gridDim.x * kThreads * kTokens;
+  for (int64_t t0 = ((int64_t)blockIdx.x * kThreads + threadIdx.x) * kTokens; t0 < a.tokens; t0 += step) {
+    const int32_t* from[kTokens];
+    int32_t* enter[kTokens];
+    int in_page[kTokens], place[kTokens];
+    int r = t0 < end ? find(cu, a.batch, (int)t0) : 0;
+#pragma unroll
+    for (int k = 0; k < kTokens; ++k) {
+      const int64_t t = t0 + k;
+      from[k] = enter[k] = nullptr;
+      place[k] = 0;
+      if (t >= end) continue;
+      while (t >= cu[r + 1]) ++r;
+      if (base[r] < 0) continue;
+      place[k] = old[r] + (int)t - cu[r];
+      const int column = fast_div(place[k], a.by_page), have = fast_div(old[r] + page - 1, a.by_page);
+      in_page[k] = place[k] - column * page;
+      int32_t* const entry = a.table + r * a.s_table + column;
+      from[k] = column < have ? entry : a.stack + (count - 1 - (base[r] + column - have));
+      if (column >= have && in_page[k] == 0) enter[k] = entry;
     }
-    a.slots[t] = slot;
-    a.positions[t] = position;
+    int id[kTokens];
+#pragma unroll
+    for (int k = 0; k < kTokens; ++k) id[k] = from[k] != nullptr ? *from[k] : -1;
+#pragma unroll
+    for (int k = 0; k < kTokens; ++k) {
+      if (t0 + k >= a.tokens) break;
+      if (enter[k] != nullptr) *enter[k] = id[k];
+      a.slots[t0 + k] = id[k] < 0 ? -1 : (int64_t)id[k] * page + in_page[k];
+      a.positions[t0 + k] = place[k];
+    }
+  }
+  if (blockIdx.x == 0) {
+    for (int r = threadIdx.x; r <= a.batch; r += kThreads) {
+      a.cu[r] = cu[r];
+      if (r < a.batch) a.granted[r] = base[r] >= 0;
+    }
   }
   if (last_workgroup(a)) {
-    for (int r = threadIdx.x; r < a.batch; r += kThreads)
-      a.lens[r] = base[r] < 0 ? old[r] : old[r] + (cu[r + 1] - cu[r]);
-    if (threadIdx.x == 0) *a.count = count - (int)taken;
+    // what is granted are the first needs of the stack
+    __shared__ int taken;
+    if (threadIdx.x == 0) taken = 0;
+    __syncthreads();
+    for (int r = threadIdx.x; r < a.batch; r += kThreads) {
+      if (base[r] < 0) {
+        a.lens[r] = old[r];
+        continue;
+      }
+      const int grown = old[r] + cu[r + 1] - cu[r];
+      a.lens[r] = grown;
+      const int needs = fast_div(grown + page - 1, a.by_page) - fast_div(old[r] + page - 1, a.by_page);
+      if (needs > 0) atomicMax(&taken, base[r] + needs);
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) *a.count = count - taken;
   }
 }
 
 // LDS: base [batch + 1] (pages given back before), keep [batch] (tokens kept)
 __global__ void __launch_bounds__(kThreads) kv4_truncate_kernel(const TablesArgs a) {
   extern __shared__ int32_t lds[];
-  __shared__ int64_t wave_sums[kThreads / 64];
+  __shared__ uint32_t sums[kThreads / 64];
   int32_t* const base = lds;
   int32_t* const keep = base + a.batch + 1;
   const int page = a.by_page.d;
   const int64_t room = min((int64_t)a.columns * page, (int64_t)INT32_MAX - page);
   const int count = clamp_int(*a.count, 0, a.capacity);
-  int64_t before = 0;
-  for (int r0 = 0; r0 < a.batch; r0 += kThreads) {
-    const int r = r0 + threadIdx.x;
-    int held = 0, kept = 0;
-    if (r < a.batch) {
-      held = clamp_int(a.lens[r], 0, room);
-      kept = clamp_int(a.change[r], 0, held);
-    }
-    int64_t total;
-    const int back = fast_div(held + page - 1, a.by_page) - fast_div(kept + page - 1, a.by_page);
-    const int64_t first = before + scan(back, wave_sums, total);
-    before += total;
-    if (r < a.batch) {
-      base[r] = clamp_int(first, 0, INT32_MAX);
-      keep[r] = kept;
-      if (r == a.batch - 1) base[a.batch] = clamp_int(first + back, 0, INT32_MAX);
-    }
+  const int each = (a.batch + kThreads - 1) / kThreads, r0 = threadIdx.x * each, r1 = min(r0 + each, a.batch);
+  uint32_t mine = 0;
+  for (int r = r0; r < r1; ++r) {
+    const int held = clamp_int(a.lens[r], 0, room), kept = clamp_int(a.change[r], 0, held);
+    keep[r] = kept;
+    base[r] = fast_div(held + page - 1, a.by_page) - fast_div(kept + page - 1, a.by_page);
+    mine = __builtin_elementwise_add_sat(mine, (uint32_t)base[r]);
   }
+  uint32_t first = scan_before(mine, sums);
+  for (int r = r0; r < r1; ++r) {
+    const int back = base[r];
+    base[r] = (int)min(first, (uint32_t)INT32_MAX);
+    first = __builtin_elementwise_add_sat(first, (uint32_t)back);
+  }
+  if (r1 == a.batch && r0 < r1) base[a.batch] = (int)min(first, (uint32_t)INT32_MAX);
   __syncthreads();
   const int total = base[a.batch];
   for (int64_t g = (int64_t)blockIdx.x * kThreads + threadIdx.x; g < total; g += (int64_t)gridDim.x * kThreads) {
@@ -250,12 +272,15 @@ int launch_kv4_tables(const tilemix_kv4_tables_params& p, bool extend, hipStream
   a.capacity = p.free_capacity;
   a.by_page = make_fast_div(p.page_size);
   if (extend) {
-    const int64_t groups = std::min<int64_t>(std::max<int64_t>((p.tokens + kThreads - 1) / kThreads, 1), 512);
+    // Every workgroup takes its turn at the ticket, so there are as few as keep one round of loads.
+    constexpr int64_t share = kThreads * kTokens;
+    const int64_t groups = std::min<int64_t>(std::max<int64_t>((p.tokens + share - 1) / share, 1), 256);
     const size_t bytes = (3 * (size_t)p.batch + 1) * sizeof(int32_t);
     hipLaunchKernelGGL(kv4_extend_kernel, dim3((unsigned)groups), dim3(kThreads), bytes, stream, a);
   } else {
-    // The pages that go back are known on the device only; most calls give back few.
-    const int64_t groups = std::min<int64_t>(std::max<int64_t>(((int64_t)p.batch * p.table_columns) / 8192, 1), 64);
+    // The pages that go back are known on the device only: at most all entries of the table.
+    const int64_t entries = (int64_t)p.batch * p.table_columns;
+    const int64_t groups = std::min<int64_t>(std::max<int64_t>((entries + kThreads - 1) / kThreads, 1), 64);
     const size_t bytes = (2 * (size_t)p.batch + 1) * sizeof(int32_t);
     hipLaunchKernelGGL(kv4_truncate_kernel, dim3((unsigned)groups), dim3(kThreads), bytes, stream, a);
   }
