@@ -990,6 +990,34 @@ struct Plan {
   int64_t bytes;
 };
 
+// Tiles of a split.  A split costs the join (a second launch, 4 us) and each workgroup's start and end (3 us, 10
+// with the chunk kernel, of which two fit a CU); too few leave the card waiting for the longest sequence.
+// Calls in us (head_dim 128, 24/8 heads unless said), this rule / others:
+//   * up to 12 tiles one: 1 x 700 (14/2 heads x 64) 8.2, split 9.5; 16 x 512 10.0 / 11.8;
+//   * few (sequence, head) pairs: two workgroups a CU.  1 x 131072 in 64 42.4, 48 45.7, 96 46.6; 3 of 2000 .. 30000
+//     in 21 30.1, 16 34.7, 32 31.1; 1 x 1024 in four 11.5, one 12.9;
+//   * else 16 tiles each (four a wave), as lengths differ and the longest sequence is waited for: 24 of 700 ..
+//     9001 (28/4 heads) in 9 29.6, 6 36.3; 24 of 61 .. 5000 in 5 29.4, 3 36.8; 16 of 61 .. 5000 in 5 25.6, 7
+//     26.1; 32 x 1024 in one 14.7, two 18.5;
+//   * but no more than three workgroups a CU, all that are resident: 64 x 8192 in one 126, two 131, four
+//     134; 48 of 200 .. 6000 in two 62.4, four 67.2; 32 x 4096 in three 42.8, four 44.2.
+int64_t plan_split(int64_t items, int64_t tiles, int block_rows) {
+  if (block_rows == kChunkRows) {
+    const int64_t splits = std::min(std::max<int64_t>(512 / items, 1), std::max<int64_t>(tiles / 8, 1));
+    return (tiles + splits - 1) / splits;
+  }
+  if (tiles <= 12) return tiles;
+  int64_t splits;
+  if (items < 64) {
+    splits = std::min(512 / items, tiles / 4);
+  } else {
+    splits = (tiles + 15) / 16;
+    if (items * splits >= 1024) splits = std::max<int64_t>(768 / items, 1);
+  }
+  const int64_t each = (tiles + splits - 1) / splits;
+  return (each + kWaves - 1) / kWaves * kWaves;  // the waves take whole tiles in turn
+}
+
 bool make_plan(const char* what, const tilemix_kv4_attn_params& p, Plan& plan) {
   if (!kv4_pool_ok(what, p.k_codes, p.k_params, p.v_codes, p.v_params, p.pages, p.page_size, p.heads_k, p.head_dim,
                    p.dtype))
@@ -1006,9 +1034,7 @@ bool make_plan(const char* what, const tilemix_kv4_attn_params& p, Plan& plan) {
   const int64_t keys = std::min<int64_t>(p.max_seqlen_k, (int64_t)p.table_columns * p.page_size);
   const int64_t tiles = std::max<int64_t>((keys + kTile - 1) / kTile, 1);
   const int64_t items = std::max<int64_t>(blocks * p.heads_k * p.batch, 1);
-  const int64_t wanted = std::max<int64_t>(1, (int64_t)(plan.block_rows < kChunkRows ? 1024 : 512) / items);
-  int64_t split_tiles = (tiles + wanted - 1) / wanted;
-  if (plan.block_rows < kChunkRows) split_tiles = (split_tiles + kWaves - 1) / kWaves * kWaves;
+  const int64_t split_tiles = plan_split(items, tiles, plan.block_rows);
   const int64_t splits = (tiles + split_tiles - 1) / split_tiles;
   const int64_t grid = blocks * splits;
   if (rows > INT32_MAX / 2 || grid > (plan.block_rows < kChunkRows ? (1 << 24) - 1 : 65535) || items * splits > INT32_MAX / 64) {
