@@ -63,6 +63,41 @@ class Call:
         assert np.isfinite(diff).all() and (diff <= tol).all(), f"worst {np.max(diff / tol):.2f} of the tolerance"
 
 
+def want_on_gpu(c):
+    """Call.want for large calls: the same formulas in float64 on the GPU."""
+    def values(codes, params):
+        codes, params = dev(codes), dev(params).double()
+        n = torch.stack((codes & 15, codes >> 4), dim=-1).flatten(-2).double()
+        s, m = (params[..., i].repeat_interleave(P.GROUP, dim=-1) for i in (0, 1))
+        return (n * s + m).half().double()[..., :c.dim]
+
+    kp, vp = values(*c.pool[:2]), values(*c.pool[2:])
+    pages, hk, page = kp.shape[:3]
+    q = dev(c.q)
+    out, mag, size = torch.zeros_like(q), torch.zeros_like(q), torch.zeros(q.shape[:2], dtype=torch.float64).cuda()
+    for b, n in enumerate(c.lens):
+        rows = slice(int(c.cu[b]), int(c.cu[b + 1]))
+        nq = rows.stop - rows.start
+        if n == 0 or nq == 0:
+            continue
+        ids = dev(c.table[b, :-(-n // page)]).long()
+        ok = (ids >= 0) & (ids < pages)
+        safe = ids.clamp(0, pages - 1)
+        there = ok.repeat_interleave(page)[:n]
+        limit = torch.arange(n - nq, n).cuda() if c.causal else torch.full((nq,), n - 1).cuda()
+        seen = there[None, :] & (torch.arange(n).cuda()[None, :] <= limit[:, None])
+        for h in range(q.shape[1]):
+            k, v = (x[safe, h // (q.shape[1] // hk)].reshape(-1, c.dim)[:n] * there[:, None] for x in (kp, vp))
+            s = (q[rows, h] @ k.T * c.scale).masked_fill(~seen, float("-inf"))
+            top = s.amax(-1, keepdim=True)
+            p = torch.exp(s - torch.where(top.isinf(), 0.0, top))
+            p = p / p.sum(-1, keepdim=True).clamp(min=1e-300)
+            out[rows, h], mag[rows, h] = p @ v, p @ v.abs()
+            size[rows, h] = (q[rows, h].abs() @ k.abs().T * abs(c.scale)).masked_fill(~seen, 0.0).amax(-1)
+    ref, mag, size = (x.cpu().numpy() for x in (out, mag, size))
+    return ref, tolerance(ref, mag, size, c.dim, c.dtype)
+
+
 # ---- page tables -------------------------------------------------------------------
 
 
@@ -283,6 +318,84 @@ def test_chunks(new, dim, heads, kv_heads, dtype):
                                                          ([6001], [4], 6, 1, 96), ([4097, 700], [40, 3], 2, 1, 32)])
 def test_long_sequences_are_split(lens, new, heads, kv_heads, dim):
     Call(lens, new, heads, kv_heads, dim, page=64, seed=dim).check()
+
+
+CHUNKS = {  # more than 96 rows a (sequence, KV head) and 10000 tiles of 32 rows: operands shared by the workgroup
+    "one": dict(lens=[6003], new=[1200], heads=3, kv_heads=1, dim=128, page=64),
+    "ragged": dict(lens=[5000, 33, 1207, 64, 0, 700], new=[700, 33, 5, 1, 0, 699], heads=6, kv_heads=2, dim=128, page=32),
+    "d64_bf16": dict(lens=[3001, 3000], new=[500, 1], heads=14, kv_heads=2, dim=64, page=16, dtype="bf16"),
+    "d96": dict(lens=[2900, 100], new=[900, 100], heads=8, kv_heads=2, dim=96, page=48),
+    "d40": dict(lens=[6000], new=[999], heads=8, kv_heads=2, dim=40, page=128, dtype="bf16"),
+    "d32": dict(lens=[4100, 64], new=[600, 200], heads=8, kv_heads=2, dim=32, page=16),
+    "all_see": dict(lens=[2500, 65], new=[1000, 3], heads=4, kv_heads=2, dim=128, page=64, causal=False),
+    "more_queries_than_keys": dict(lens=[1500, 900], new=[2000, 901], heads=4, kv_heads=2, dim=128, page=64),
+    "split": dict(lens=[70000, 60000], new=[45, 33], heads=3, kv_heads=1, dim=128, page=64),
+    "split_bf16_d64": dict(lens=[70001], new=[60], heads=7, kv_heads=1, dim=64, page=64, dtype="bf16"),
+}
+
+
+@pytest.mark.parametrize("name", CHUNKS)
+def test_chunk_kernel(name):
+    c = Call(seed=len(name), **CHUNKS[name])
+    hk, rows = c.pool[0].shape[1], c.max_q * c.q.shape[1] // c.pool[0].shape[1]
+    assert rows > 96 and -(-rows // 32) * hk * len(c.lens) * -(-c.max_k // 64) > 10000
+    got = c.run()
+    ref, tol = want_on_gpu(c)
+    diff = np.abs(got.double().cpu().numpy() - ref)
+    assert np.isfinite(diff).all() and (diff <= tol).all(), f"worst {np.max(diff / tol):.2f} of the tolerance"
+
+
+def test_chunk_kernel_pages_nan_and_what_lies_behind():
+    """Bad pages, stale rows behind the end and a stored NaN, with operands shared by the workgroup."""
+    c = Call([3000, 700], [1000, 40], 6, 2, 128, page=16, seed=21)
+    ref, tol = want_on_gpu(c)
+    clean = c.run().double().cpu().numpy()
+    assert (np.abs(clean - ref) <= tol).all()
+    used = np.zeros(c.pool[0].shape[0] * 16, dtype=bool)
+    for b, n in enumerate(c.lens):
+        for t in range(n):
+            used[int(c.table[b, t // 16]) * 16 + t % 16] = True
+    used = used.reshape(-1, 16)
+    for at in (1, 3):
+        c.pool[at][~used.repeat(2, axis=0).reshape(-1, 2, 16)] = np.nan
+    assert np.array_equal(c.run().double().cpu().numpy(), clean)
+    # V of KV head 1, group 1, key 2500 of sequence 0: queries from 500 on see it
+    c.pool[3][c.table[0, 2500 // 16], 1, 2500 % 16, 1, 0] = np.nan
+    got = c.run().double().cpu().numpy()
+    want = clean.copy()
+    want[500:1000, 3:, 32:64] = np.nan
+    assert np.array_equal(np.isnan(got), np.isnan(want))
+    assert np.array_equal(got[~np.isnan(want)], clean[~np.isnan(want)])
+    c = Call([3000, 700], [1000, 40], 6, 2, 128, page=16, seed=21)
+    c.table[0, 3], c.table[0, 100], c.table[0, 187] = -1, 10 ** 9, -2 ** 31
+    c.table[1, :] = -7
+    ref, tol = want_on_gpu(c)
+    got = c.run().double().cpu().numpy()
+    assert (np.abs(got - ref) <= tol).all() and not got[1000:].any()
+
+
+def test_chunk_kernel_out_and_graph():
+    """Strided q and out, rows behind the last query, one captured call replayed on changed inputs."""
+    c = Call([2600, 100], [900, 3], 6, 2, 128, page=64, seed=22)
+    q, *rest = c.device_args()
+    clean = paged_int4_attention(q, *rest)
+    wide = torch.zeros(910, 6, 133, dtype=torch.float16, device="cuda")
+    wide[:903, :, 3:131] = q
+    out = torch.full((6, 910, 140), 9.0, dtype=torch.float16, device="cuda").transpose(0, 1)
+    paged_int4_attention(wide[:, :, 3:131], *rest, out=out[:, :, 5:133])
+    assert torch.equal(out[:903, :, 5:133], clean)
+    assert (out[903:] == 9.0).all() and (out[:, :, :5] == 9.0).all() and (out[:, :, 133:] == 9.0).all()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = paged_int4_attention(q, *rest)
+    lens = rest[2]
+    for step in range(3):
+        q.copy_(torch.randn(q.shape, generator=torch.Generator().manual_seed(step)).half())
+        lens.copy_(ints([2600 - 300 * step, 100 - step]))
+        want = paged_int4_attention(q, *rest)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(captured, want)
 
 
 @pytest.mark.parametrize("scale", [0.0, -0.2, 0.5, 1e-30])

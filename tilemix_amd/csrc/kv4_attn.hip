@@ -1029,10 +1029,16 @@ bool make_plan(const char* what, const tilemix_kv4_attn_params& p, Plan& plan) {
     return false;
   }
   const int64_t rows = (int64_t)p.max_seqlen_q * (p.heads_q / p.heads_k);
-  plan.block_rows = rows <= 16 ? 16 : rows <= 32 ? 32 : kChunkRows;
-  const int64_t blocks = (rows + plan.block_rows - 1) / plan.block_rows;
   const int64_t keys = std::min<int64_t>(p.max_seqlen_k, (int64_t)p.table_columns * p.page_size);
   const int64_t tiles = std::max<int64_t>((keys + kTile - 1) / kTile, 1);
+  // The chunk kernel needs rows to share its conversions among, and work that outweighs its start and end; the
+  // other one takes the same rows 32 at a time.  Calls in us, blocks of 32 / chunk kernel (24/8 heads x 128, tiles
+  // of blocks of 32): 90 rows 8 x 4000 41.3 / 42.6; 120 rows 1 x 4000 (2016) 17.5 / 29.5, 8 x 4000 (16128) 51.4 /
+  // 44.2, 1 x 40000 (20000) 49.5 / 47.0; 300 rows 1 x 4000 (5040) 28.4 / 31.4, 1 x 40000 (50000) 111 / 88.
+  const int64_t blocks32 = (rows + 31) / 32;
+  const bool few = blocks32 * p.heads_k * p.batch * tiles <= 10000;
+  plan.block_rows = rows <= 16 ? 16 : rows <= 96 || few ? 32 : kChunkRows;
+  const int64_t blocks = (rows + plan.block_rows - 1) / plan.block_rows;
   const int64_t items = std::max<int64_t>(blocks * p.heads_k * p.batch, 1);
   const int64_t split_tiles = plan_split(items, tiles, plan.block_rows);
   const int64_t splits = (tiles + split_tiles - 1) / split_tiles;

@@ -38,12 +38,15 @@ struct RowsArgs {
   FastDiv by_page;
 };
 
-// Thread = one word (eight channels) of a row: 4 NG threads a row, so that a wave reads
-// whole rows in 16-byte pieces and the four lanes of a group find its range among them.
+// Thread = one word (eight channels) of the K and the V row of kPer tokens: 4 NG threads a row, so that a
+// wave reads whole rows in 16-byte pieces and the four lanes of a group find its range among them.  A
+// thread's loads are all in flight together, behind one look at the token's place: bound by those two latencies a
+// round before by bytes (16384 tokens of 8 heads x 128, one row a thread: store 33 us, load 25).
 template <int NG>
 struct RowSplit {
   static constexpr int kWords = 4 * NG;
-  static constexpr int kRows = 256 / kWords;  // of a workgroup (NG = 3: the last four threads idle)
+  static constexpr int kRows = 256 / kWords;  // at a time (NG = 3: the last four threads idle)
+  static constexpr int kPer = 2;
 };
 
 __device__ __forceinline__ float quad_xor1(float x) {
@@ -53,116 +56,175 @@ __device__ __forceinline__ float quad_xor2(float x) {
   return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x), 0x4e, 0xf, 0xf, true));
 }
 
+// Eight values; those behind `there` are copies of the first, which the group's range does not notice.
 template <typename T>
-__device__ __forceinline__ f32x8 read8(const T* x, int count, bool vec) {
-  typedef T T8 __attribute__((ext_vector_type(8)));
-  if (vec && count >= 8) return __builtin_convertvector(*reinterpret_cast<const T8*>(x), f32x8);
-  f32x8 v = {};
+__device__ __forceinline__ u32x4 read8(const T* x, int there, bool vec) {
+  if (vec && there >= 8) return *reinterpret_cast<const u32x4*>(x);
+  const uint16_t* const from = reinterpret_cast<const uint16_t*>(x);
+  u32x4 v;
 #pragma unroll
-  for (int e = 0; e < 8; ++e)
-    if (e < count) v[e] = (float)x[e];
+  for (int e = 0; e < 4; ++e) {
+    const uint32_t lo = from[2 * e < there ? 2 * e : 0], hi = from[2 * e + 1 < there ? 2 * e + 1 : 0];
+    v[e] = lo | hi << 16;
+  }
   return v;
 }
 
-template <int NG, typename T>
-__global__ void __launch_bounds__(256) kv4_store_kernel(const RowsArgs a) {
-  using S = RowSplit<NG>;
-  const int r = threadIdx.x / S::kWords, w = threadIdx.x - r * S::kWords, h = blockIdx.y, z = blockIdx.z;
-  const int64_t t = (int64_t)blockIdx.x * S::kRows + r;
-  if (r >= S::kRows || t >= a.tokens) return;
-  const int64_t slot = a.slots[t];
-  if (slot < 0 || slot >= (int64_t)a.pages * a.by_page.d) return;
-  const int there = min(8, a.d - 8 * w);  // channels of this word
-  const T* x = static_cast<const T*>(a.x[z]) + t * a.st[z] + h * a.sh[z] + 8 * w;
-  f32x8 v = read8(x, there, a.vec);
-  float lo = __builtin_inff(), hi = -__builtin_inff();
+__device__ __forceinline__ void widen(const u32x4& raw, f16, f32x8& v) {
+  v = __builtin_convertvector(__builtin_bit_cast(f16x8, raw), f32x8);
+}
+__device__ __forceinline__ void widen(const u32x4& raw, bf16, f32x8& v) {
+  v = __builtin_convertvector(__builtin_bit_cast(bf16x8, raw), f32x8);
+}
+
+// The codes of a word of eight channels and, in every lane of the group, the group's parameters.
+template <typename T>
+__device__ __forceinline__ uint32_t quantise8(const u32x4& raw, bool present, uint32_t& param) {
+  f32x8 v;
+  widen(raw, T(), v);
+  float lo = v[0], hi = v[0];
   bool nan = false;
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    nan |= e < there && v[e] != v[e];
-    v[e] = fminf(fmaxf(v[e], -kKv4Limit), kKv4Limit);
-    if (e < there) {
-      lo = fminf(lo, v[e]);
-      hi = fmaxf(hi, v[e]);
-    }
+    nan |= v[e] != v[e];
+    lo = fminf(lo, v[e]);
+    hi = fmaxf(hi, v[e]);
   }
-  // (the four lanes of a group are in or out together: rows of four words each group)
+  // (the four lanes of a group are in or out together; a word behind the last channel has no say)
+  lo = present ? lo : __builtin_inff();
+  hi = present ? hi : -__builtin_inff();
+  float bad = nan && present ? 1.0f : 0.0f;
   lo = fminf(lo, quad_xor1(lo));
   hi = fmaxf(hi, quad_xor1(hi));
+  bad = fmaxf(bad, quad_xor1(bad));
   lo = fminf(lo, quad_xor2(lo));
   hi = fmaxf(hi, quad_xor2(hi));
-  float bad = nan ? 1.0f : 0.0f;
-  bad = fmaxf(bad, quad_xor1(bad));
   bad = fmaxf(bad, quad_xor2(bad));
+  lo = fminf(fmaxf(lo, -kKv4Limit), kKv4Limit);
+  hi = fminf(fmaxf(hi, -kKv4Limit), kKv4Limit);
   f16 s = (f16)((hi - lo) / 15.0f), m = (f16)lo;
   if (bad != 0.0f) {
     s = (f16)0.0f;
     m = (f16)__builtin_nanf("");
   }
-  const float step = (float)s, least = (float)m;
-  uint32_t word = 0;
-  if (step > 0.0f) {
+  param = (uint32_t)__builtin_bit_cast(uint16_t, s) | (uint32_t)__builtin_bit_cast(uint16_t, m) << 16;
+  // (x - m) / s as an IEEE division rounds it, from the rounded reciprocal: Markstein's correction of the
+  // quotient.  (s >= 2^-24 and quotients below 2^6 leave no step to underflow.)  Adding 1.5 2^23 rounds to a whole
+  // number in the low bits; the sum of the shifted results counts that constant's bits once a code.
+  const float step = (float)s, least = (float)m, recip = 1.0f / step;
+  constexpr uint32_t kMagic = 0x4b400000u;
+  uint32_t word = 0u - (kMagic + (kMagic << 4) + (kMagic << 8) + (kMagic << 12) + (kMagic << 16) + (kMagic << 20) +
+                        (kMagic << 24) + (kMagic << 28));
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float n = fminf(fmaxf(rintf((v[e] - least) / step), 0.0f), 15.0f);
-      if (e < there) word |= (uint32_t)n << (4 * e);
+  for (int e = 0; e < 8; ++e) {
+    const float x = fminf(fmaxf(v[e], -kKv4Limit), kKv4Limit) - least;
+    const float q = x * recip;
+    const float n = __builtin_fmaf(__builtin_fmaf(-q, step, x), recip, q);
+    word += __builtin_bit_cast(uint32_t, fminf(fmaxf(n, 0.0f), 15.0f) + 12582912.0f) << (4 * e);
+  }
+  return step > 0.0f ? word : 0u;
+}
+
+template <int NG, typename T>
+__global__ void __launch_bounds__(256) kv4_store_kernel(const RowsArgs a) {
+  using S = RowSplit<NG>;
+  const int r = threadIdx.x / S::kWords, w = threadIdx.x - r * S::kWords, h = blockIdx.y;
+  const int64_t t0 = (int64_t)blockIdx.x * (S::kRows * S::kPer) + r;
+  const int there = min(8, a.d - 8 * w);  // channels of this word
+  if (r >= S::kRows || t0 >= a.tokens) return;
+  int64_t slot[S::kPer];
+  u32x4 raw[S::kPer][2];
+#pragma unroll
+  for (int k = 0; k < S::kPer; ++k) {
+    const int64_t t = min(t0 + k * S::kRows, a.tokens - 1);
+    slot[k] = a.slots[t];
+#pragma unroll
+    for (int z = 0; z < 2; ++z)  // (a word behind the last channel reads the row's first)
+      raw[k][z] = read8(static_cast<const T*>(a.x[z]) + t * a.st[z] + h * a.sh[z] + (there > 0 ? 8 * w : 0),
+                        there > 0 ? there : 8, a.vec);
+  }
+#pragma unroll
+  for (int k = 0; k < S::kPer; ++k) {
+    if (t0 + k * S::kRows >= a.tokens || slot[k] < 0 || slot[k] >= (int64_t)a.pages * a.by_page.d) continue;
+    const int page = fast_div((int)slot[k], a.by_page), at = (int)slot[k] - page * a.by_page.d;
+    const int64_t row = ((int64_t)page * a.heads + h) * a.by_page.d + at;
+#pragma unroll
+    for (int z = 0; z < 2; ++z) {
+      uint32_t param, word = quantise8<T>(raw[k][z], there > 0, param);
+      if (there < 8) word &= there > 0 ? (1u << (4 * there)) - 1 : 0u;
+      a.codes[z][row * S::kWords + w] = word;
+      if ((w & 3) == 0) a.params[z][row * NG + (w >> 2)] = param;
     }
   }
-  const int page = (int)(slot / a.by_page.d), at = (int)(slot - (int64_t)page * a.by_page.d);
-  const int64_t row = ((int64_t)page * a.heads + h) * a.by_page.d + at;
-  a.codes[z][row * S::kWords + w] = word;
-  if ((w & 3) == 0)
-    a.params[z][row * NG + (w >> 2)] =
-        (uint32_t)__builtin_bit_cast(uint16_t, s) | (uint32_t)__builtin_bit_cast(uint16_t, m) << 16;
 }
 
 template <int NG, typename T>
 __global__ void __launch_bounds__(256) kv4_load_kernel(const RowsArgs a) {
   using S = RowSplit<NG>;
   typedef T T8 __attribute__((ext_vector_type(8)));
-  const int r = threadIdx.x / S::kWords, w = threadIdx.x - r * S::kWords, h = blockIdx.y, z = blockIdx.z;
-  const int64_t t0 = (int64_t)blockIdx.x * S::kRows, t = t0 + r;
-  // The sequence that ends behind the workgroup's first row: entries 1 .. batch - 1 of cu at or before it.
+  const int r = threadIdx.x / S::kWords, w = threadIdx.x - r * S::kWords, h = blockIdx.y;
+  const int64_t first = (int64_t)blockIdx.x * (S::kRows * S::kPer);
+  // The sequence that holds the workgroup's first row: entries 1 .. batch - 1 of cu at or before it.
   int b = 0;
   for (int i = 1 + (threadIdx.x & 63); i - (int)(threadIdx.x & 63) < a.batch; i += 64)
-    b += __popcll(__ballot(i < a.batch && a.cu[i] <= t0));
-  if (r >= S::kRows || t >= a.tokens) return;
-  while (b + 1 < a.batch && a.cu[b + 1] <= t) ++b;
-  const int64_t start = a.cu[b];
-  int64_t row = -1;
-  if (t >= start && t < a.cu[b + 1]) {
-    const int at = (int)(t - start), column = fast_div(at, a.by_page);
-    const int page = column < a.columns ? a.table[b * a.s_table + column] : -1;
-    if (page >= 0 && page < a.pages) row = ((int64_t)page * a.heads + h) * a.by_page.d + at - column * a.by_page.d;
-  }
-  f16x2 v[4] = {};
-  if (row >= 0) {
-    const uint32_t p = a.params[z][row * NG + (w >> 2)];
-    const f16x2 sm = __builtin_bit_cast(f16x2, p), s = {sm[0], sm[0]}, m = {sm[1], sm[1]};
-    kv4_codes(a.codes[z][row * S::kWords + w], v);
+    b += __popcll(__ballot(i < a.batch && a.cu[i] <= first));
+  const int64_t t0 = first + r;
+  if (r >= S::kRows || t0 >= a.tokens) return;
+  int64_t row[S::kPer];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) v[i] = kv4_fma(v[i], s, m);
+  for (int k = 0; k < S::kPer; ++k) {
+    const int64_t t = t0 + k * S::kRows;
+    while (b + 1 < a.batch && a.cu[b + 1] <= t) ++b;
+    row[k] = -1;
+    if (t < a.tokens && t >= a.cu[b] && t < a.cu[b + 1]) {
+      const int at = (int)t - a.cu[b], column = fast_div(at, a.by_page);
+      const int page = column < a.columns ? a.table[b * a.s_table + column] : -1;
+      if (page >= 0 && page < a.pages) row[k] = ((int64_t)page * a.heads + h) * a.by_page.d + at - column * a.by_page.d;
+    }
   }
-  T8 out;
+  uint32_t word[S::kPer][2], param[S::kPer][2];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    out[i] = (T)(float)v[i][0];
-    out[i + 4] = (T)(float)v[i][1];
-  }
-  T* x = static_cast<T*>(a.x[z]) + t * a.st[z] + h * a.sh[z] + 8 * w;
+  for (int k = 0; k < S::kPer; ++k)
+#pragma unroll
+    for (int z = 0; z < 2; ++z) {  // (no row: the pool's first, for nothing)
+      const int64_t from = max(row[k], (int64_t)0);
+      word[k][z] = a.codes[z][from * S::kWords + w];
+      param[k][z] = a.params[z][from * NG + (w >> 2)];
+    }
   const int there = min(8, a.d - 8 * w);
-  if (a.vec && there == 8) {
-    *reinterpret_cast<T8*>(x) = out;
-  } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (e < there) x[e] = out[e];
+  for (int k = 0; k < S::kPer; ++k) {
+    const int64_t t = t0 + k * S::kRows;
+    if (t >= a.tokens) continue;
+#pragma unroll
+    for (int z = 0; z < 2; ++z) {
+      const uint32_t p = row[k] >= 0 ? param[k][z] : 0u;
+      const f16x2 sm = __builtin_bit_cast(f16x2, p), s = {sm[0], sm[0]}, m = {sm[1], sm[1]};
+      f16x2 v[4];
+      kv4_codes(word[k][z], v);
+      T8 out;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v[i] = kv4_fma(v[i], s, m);
+        out[i] = (T)(float)v[i][0];
+        out[i + 4] = (T)(float)v[i][1];
+      }
+      T* x = static_cast<T*>(a.x[z]) + t * a.st[z] + h * a.sh[z] + 8 * w;
+      if (a.vec && there == 8) {
+        *reinterpret_cast<T8*>(x) = out;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (e < there) x[e] = out[e];
+      }
+    }
   }
 }
 
 template <int NG>
 void launch_rows(const RowsArgs& a, bool store, bool bf, hipStream_t stream) {
-  const dim3 grid((unsigned)((a.tokens + RowSplit<NG>::kRows - 1) / RowSplit<NG>::kRows), a.heads, 2), block(256);
+  constexpr int rows = RowSplit<NG>::kRows * RowSplit<NG>::kPer;
+  const dim3 grid((unsigned)((a.tokens + rows - 1) / rows), a.heads), block(256);
   if (store && bf) hipLaunchKernelGGL((kv4_store_kernel<NG, bf16>), grid, block, 0, stream, a);
   else if (store) hipLaunchKernelGGL((kv4_store_kernel<NG, f16>), grid, block, 0, stream, a);
   else if (bf) hipLaunchKernelGGL((kv4_load_kernel<NG, bf16>), grid, block, 0, stream, a);
