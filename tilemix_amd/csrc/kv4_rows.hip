@@ -4,6 +4,7 @@
 #include "kv4_common.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace tmx {
 
@@ -38,16 +39,23 @@ struct RowsArgs {
   FastDiv by_page;
 };
 
-// Thread = one word (eight channels) of the K and the V row of kPer tokens: 4 NG threads a row, so that a
-// wave reads whole rows in 16-byte pieces and the four lanes of a group find its range among them.  A
-// thread's loads are all in flight together, behind one look at the token's place: bound by those two latencies a
-// round before by bytes (16384 tokens of 8 heads x 128, one row a thread: store 33 us, load 25).
+// Thread = one word (eight channels) of the K and the V row of a token (load: of kPer tokens): 4 NG threads a
+// row, so that a wave reads whole rows in 16-byte pieces and the four lanes of a group find its range among
+// them.  A thread's loads are all in flight together, behind one look at the token's place.
+// 16384 tokens of 8 heads x 128, 88 MB each way: load 16.4 us (5.4 TB/s, a large copy's rate; K and V by threads of
+// their own 25), store 21.4 (4.1 TB/s, its 110 vector instructions a word take about 13 of it; IEEE divisions 33).
 template <int NG>
 struct RowSplit {
   static constexpr int kWords = 4 * NG;
   static constexpr int kRows = 256 / kWords;  // at a time (NG = 3: the last four threads idle)
   static constexpr int kPer = 2;
 };
+
+// An fp32 result as such: its conversion to fp16 is a rounding of its own, which the compiler would fuse.
+__device__ __forceinline__ float keep32(float x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
 
 __device__ __forceinline__ float quad_xor1(float x) {
   return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x), 0xb1, 0xf, 0xf, true));
@@ -70,29 +78,87 @@ __device__ __forceinline__ u32x4 read8(const T* x, int there, bool vec) {
   return v;
 }
 
-__device__ __forceinline__ void widen(const u32x4& raw, f16, f32x8& v) {
-  v = __builtin_convertvector(__builtin_bit_cast(f16x8, raw), f32x8);
-}
-__device__ __forceinline__ void widen(const u32x4& raw, bf16, f32x8& v) {
-  v = __builtin_convertvector(__builtin_bit_cast(bf16x8, raw), f32x8);
+// Smallest and largest of eight values, and all of them less a number in fp32, rounded once.  (NaNs are looked for
+// elsewhere.)
+struct Eight16 {
+  f16x2 v[4];
+  __device__ __forceinline__ Eight16(const u32x4& raw) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t pair = raw[e];
+      v[e] = __builtin_bit_cast(f16x2, pair);
+    }
+  }
+  __device__ __forceinline__ float least() const {
+    const f16x2 x = __builtin_elementwise_min(__builtin_elementwise_min(v[0], v[1]), __builtin_elementwise_min(v[2], v[3]));
+    return fminf((float)x[0], (float)x[1]);
+  }
+  __device__ __forceinline__ float most() const {
+    const f16x2 x = __builtin_elementwise_max(__builtin_elementwise_max(v[0], v[1]), __builtin_elementwise_max(v[2], v[3]));
+    return fmaxf((float)x[0], (float)x[1]);
+  }
+  __device__ __forceinline__ void cap() {
+    const f16x2 top = {(f16)kKv4Limit, (f16)kKv4Limit};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = __builtin_elementwise_min(v[e], top);
+  }
+  __device__ __forceinline__ float less(int e, float m) const {
+    const uint32_t pair = __builtin_bit_cast(uint32_t, v[e >> 1]);
+    return e & 1 ? sub_hi(pair, -m) : sub_lo(pair, -m);
+  }
+};
+struct EightBf16 {
+  float v[8];
+  __device__ __forceinline__ EightBf16(const u32x4& raw) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t pair = raw[e];
+      v[2 * e] = __uint_as_float(pair << 16);
+      v[2 * e + 1] = __uint_as_float(pair & 0xffff0000u);
+    }
+  }
+  __device__ __forceinline__ float least() const {
+    float x = v[0];
+#pragma unroll
+    for (int e = 1; e < 8; ++e) x = fminf(x, v[e]);
+    return x;
+  }
+  __device__ __forceinline__ float most() const {
+    float x = v[0];
+#pragma unroll
+    for (int e = 1; e < 8; ++e) x = fmaxf(x, v[e]);
+    return x;
+  }
+  __device__ __forceinline__ void cap() {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = fminf(v[e], kKv4Limit);
+  }
+  __device__ __forceinline__ float less(int e, float m) const { return v[e] - m; }
+};
+
+// x / y as an IEEE division rounds it, from the correctly rounded reciprocal r of y: Markstein's correction of the
+// quotient (no step underflows for the y >= 2^-24 and quotients below 2^18 here).
+__device__ __forceinline__ float divide(float x, float y, float r) {
+  const float q = x * r;
+  return __builtin_fmaf(__builtin_fmaf(-q, y, x), r, q);
 }
 
 // The codes of a word of eight channels and, in every lane of the group, the group's parameters.
 template <typename T>
 __device__ __forceinline__ uint32_t quantise8(const u32x4& raw, bool present, uint32_t& param) {
-  f32x8 v;
-  widen(raw, T(), v);
-  float lo = v[0], hi = v[0];
-  bool nan = false;
+  typename std::conditional<std::is_same<T, f16>::value, Eight16, EightBf16>::type v(raw);
+  constexpr uint32_t kInf = std::is_same<T, f16>::value ? 0x7c00u : 0x7f80u;
+  typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+  u16x2 size = {};
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    nan |= v[e] != v[e];
-    lo = fminf(lo, v[e]);
-    hi = fmaxf(hi, v[e]);
+  for (int e = 0; e < 4; ++e) {
+    const uint32_t pair = raw[e] & 0x7fff7fffu;
+    size = __builtin_elementwise_max(size, __builtin_bit_cast(u16x2, pair));
   }
+  const bool nan = size[0] > kInf || size[1] > kInf;
   // (the four lanes of a group are in or out together; a word behind the last channel has no say)
-  lo = present ? lo : __builtin_inff();
-  hi = present ? hi : -__builtin_inff();
+  float lo = present ? v.least() : __builtin_inff();
+  float hi = present ? v.most() : -__builtin_inff();
   float bad = nan && present ? 1.0f : 0.0f;
   lo = fminf(lo, quad_xor1(lo));
   hi = fmaxf(hi, quad_xor1(hi));
@@ -100,61 +166,55 @@ __device__ __forceinline__ uint32_t quantise8(const u32x4& raw, bool present, ui
   lo = fminf(lo, quad_xor2(lo));
   hi = fmaxf(hi, quad_xor2(hi));
   bad = fmaxf(bad, quad_xor2(bad));
-  lo = fminf(fmaxf(lo, -kKv4Limit), kKv4Limit);
-  hi = fminf(fmaxf(hi, -kKv4Limit), kKv4Limit);
-  f16 s = (f16)((hi - lo) / 15.0f), m = (f16)lo;
+  lo = __builtin_amdgcn_fmed3f(lo, -kKv4Limit, kKv4Limit);
+  hi = __builtin_amdgcn_fmed3f(hi, -kKv4Limit, kKv4Limit);
+  f16 s = (f16)keep32(divide(hi - lo, 15.0f, 1.0f / 15.0f)), m = (f16)lo;
   if (bad != 0.0f) {
     s = (f16)0.0f;
     m = (f16)__builtin_nanf("");
   }
   param = (uint32_t)__builtin_bit_cast(uint16_t, s) | (uint32_t)__builtin_bit_cast(uint16_t, m) << 16;
-  // (x - m) / s as an IEEE division rounds it, from the rounded reciprocal: Markstein's correction of the
-  // quotient.  (s >= 2^-24 and quotients below 2^6 leave no step to underflow.)  Adding 1.5 2^23 rounds to a whole
-  // number in the low bits; the sum of the shifted results counts that constant's bits once a code.
-  const float step = (float)s, least = (float)m, recip = 1.0f / step;
+  // 1 / s: a Newton step on the hardware reciprocal leaves 2^-22 of a last place before its rounding, and s has 11
+  // bits: 1 / s is no nearer than 2^-12 of a last place to where two roundings meet.  So it is the right one.
+  // Adding 1.5 2^23 rounds to a whole number in the low bits; the sum of the shifted results counts that
+  // constant's bits once a code.  (Minus infinity makes a NaN here, which the median takes for the smallest: code 0.)
+  const float step = (float)s, least = (float)m, near = __builtin_amdgcn_rcpf(step);
+  const float recip = __builtin_fmaf(__builtin_fmaf(-step, near, 1.0f), near, near);
   constexpr uint32_t kMagic = 0x4b400000u;
   uint32_t word = 0u - (kMagic + (kMagic << 4) + (kMagic << 8) + (kMagic << 12) + (kMagic << 16) + (kMagic << 20) +
                         (kMagic << 24) + (kMagic << 28));
+  v.cap();
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    const float x = fminf(fmaxf(v[e], -kKv4Limit), kKv4Limit) - least;
-    const float q = x * recip;
-    const float n = __builtin_fmaf(__builtin_fmaf(-q, step, x), recip, q);
-    word += __builtin_bit_cast(uint32_t, fminf(fmaxf(n, 0.0f), 15.0f) + 12582912.0f) << (4 * e);
+    const float n = __builtin_amdgcn_fmed3f(divide(v.less(e, least), step, recip), 0.0f, 15.0f);
+    word += __builtin_bit_cast(uint32_t, n + 12582912.0f) << (4 * e);
   }
   return step > 0.0f ? word : 0u;
 }
 
+// (One token a thread: two measured 21.6 us for 16384 tokens of 8 heads x 128, four 24.5, one 21.4.)
 template <int NG, typename T>
 __global__ void __launch_bounds__(256) kv4_store_kernel(const RowsArgs a) {
   using S = RowSplit<NG>;
   const int r = threadIdx.x / S::kWords, w = threadIdx.x - r * S::kWords, h = blockIdx.y;
-  const int64_t t0 = (int64_t)blockIdx.x * (S::kRows * S::kPer) + r;
+  const int64_t t = (int64_t)blockIdx.x * S::kRows + r;
   const int there = min(8, a.d - 8 * w);  // channels of this word
-  if (r >= S::kRows || t0 >= a.tokens) return;
-  int64_t slot[S::kPer];
-  u32x4 raw[S::kPer][2];
+  if (r >= S::kRows || t >= a.tokens) return;
+  const int64_t slot = a.slots[t];
+  u32x4 raw[2];
 #pragma unroll
-  for (int k = 0; k < S::kPer; ++k) {
-    const int64_t t = min(t0 + k * S::kRows, a.tokens - 1);
-    slot[k] = a.slots[t];
+  for (int z = 0; z < 2; ++z)  // (a word behind the last channel reads the row's first)
+    raw[z] = read8(static_cast<const T*>(a.x[z]) + t * a.st[z] + h * a.sh[z] + (there > 0 ? 8 * w : 0),
+                   there > 0 ? there : 8, a.vec);
+  if (slot < 0 || slot >= (int64_t)a.pages * a.by_page.d) return;
+  const int page = fast_div((int)slot, a.by_page), at = (int)slot - page * a.by_page.d;
+  const int64_t row = ((int64_t)page * a.heads + h) * a.by_page.d + at;
 #pragma unroll
-    for (int z = 0; z < 2; ++z)  // (a word behind the last channel reads the row's first)
-      raw[k][z] = read8(static_cast<const T*>(a.x[z]) + t * a.st[z] + h * a.sh[z] + (there > 0 ? 8 * w : 0),
-                        there > 0 ? there : 8, a.vec);
-  }
-#pragma unroll
-  for (int k = 0; k < S::kPer; ++k) {
-    if (t0 + k * S::kRows >= a.tokens || slot[k] < 0 || slot[k] >= (int64_t)a.pages * a.by_page.d) continue;
-    const int page = fast_div((int)slot[k], a.by_page), at = (int)slot[k] - page * a.by_page.d;
-    const int64_t row = ((int64_t)page * a.heads + h) * a.by_page.d + at;
-#pragma unroll
-    for (int z = 0; z < 2; ++z) {
-      uint32_t param, word = quantise8<T>(raw[k][z], there > 0, param);
-      if (there < 8) word &= there > 0 ? (1u << (4 * there)) - 1 : 0u;
-      a.codes[z][row * S::kWords + w] = word;
-      if ((w & 3) == 0) a.params[z][row * NG + (w >> 2)] = param;
-    }
+  for (int z = 0; z < 2; ++z) {
+    uint32_t param, word = quantise8<T>(raw[z], there > 0, param);
+    if (there < 8) word &= there > 0 ? (1u << (4 * there)) - 1 : 0u;
+    a.codes[z][row * S::kWords + w] = word;
+    if ((w & 3) == 0) a.params[z][row * NG + (w >> 2)] = param;
   }
 }
 
@@ -223,7 +283,7 @@ __global__ void __launch_bounds__(256) kv4_load_kernel(const RowsArgs a) {
 
 template <int NG>
 void launch_rows(const RowsArgs& a, bool store, bool bf, hipStream_t stream) {
-  constexpr int rows = RowSplit<NG>::kRows * RowSplit<NG>::kPer;
+  const int rows = RowSplit<NG>::kRows * (store ? 1 : RowSplit<NG>::kPer);
   const dim3 grid((unsigned)((a.tokens + rows - 1) / rows), a.heads), block(256);
   if (store && bf) hipLaunchKernelGGL((kv4_store_kernel<NG, bf16>), grid, block, 0, stream, a);
   else if (store) hipLaunchKernelGGL((kv4_store_kernel<NG, f16>), grid, block, 0, stream, a);
