@@ -21,6 +21,7 @@ from transformers.models.llama.modeling_llama import apply_rotary_pos_emb
 
 from .. import _native
 from ..attention import precision_maps as pm
+from .int4_cache import Int4KVCache
 
 # Below this many query tokens the module falls back to its parent's attention
 # (reference models/tilemix_llama.py:527-537).
@@ -42,6 +43,19 @@ def apply_rotary(q: Tensor, k: Tensor, cos: Tensor, sin: Tensor):
         if out is not None:
             return out
     return apply_rotary_pos_emb(q, k, cos, sin)
+
+
+def int4_route(past, layer_idx: int, attention_mask, seqlen: int) -> tuple[bool, bool]:
+    """Which way a module's call takes: (attention over the 4-bit cache, the parent class's attention), neither
+    being the TileMix prefill.  Without an ``Int4KVCache`` that is the parent's below
+    ``MIN_TILEMIX_SEQLEN`` tokens; with one its first tokens are prefilled the same way, and later or fewer ones
+    attend to it, or, with a mask that it does not serve, go through the parent (which reads the cache back)."""
+    few = seqlen < MIN_TILEMIX_SEQLEN
+    if not isinstance(past, Int4KVCache):
+        return False, few
+    later = few or past.get_seq_length(layer_idx) > 0
+    serves = past.serves(attention_mask)
+    return later and serves, later and not serves
 
 
 @dataclass(frozen=True)

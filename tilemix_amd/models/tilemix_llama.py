@@ -6,7 +6,8 @@ Public surface, same names and signatures as the reference:
   routed FP16/INT8 kernel through ``tilemix_varlen_attention``;
 * ``inject_tilemix_into_llama(model)`` / ``configure_tilemix_attention_pattern``;
 * ``PrefillCache`` -- a KV cache whose first update stores the prefill K/V
-  without a copy (reference :703-715);
+  without a copy (reference :703-715); for a cache in 4 bits and the attention that goes
+  on over it see ``int4_cache.Int4KVCache``;
 * ``prepare_llama_prefill(model)`` -- prefill helpers: RMSNorm, token-major
   RoPE (so the attention entry needs no transpose copy) and SiLU*mul
   (reference :718-895), restated with torch ops at the reference's rounding
@@ -24,7 +25,7 @@ from transformers.models.llama.modeling_llama import LlamaAttention
 
 from .. import _native
 from ..attention.tilemix_varlen import tilemix_varlen_attention
-from ._common import (MIN_TILEMIX_SEQLEN, BucketConfig, TileMixRoutingMixin, apply_rotary,  # noqa: F401
+from ._common import (MIN_TILEMIX_SEQLEN, BucketConfig, TileMixRoutingMixin, apply_rotary, int4_route,  # noqa: F401
                       pick_block_n_for_64, pick_mask_block_n)
 
 __all__ = ["TileMixLlamaAttention", "inject_tilemix_into_llama", "configure_tilemix_attention_pattern", "rms_norm",
@@ -57,12 +58,14 @@ class TileMixLlamaAttention(TileMixRoutingMixin, LlamaAttention):
         bsz, seqlen, _ = hidden_states.size()
         hidden_states = self._ensure_cuda(hidden_states)
         device = hidden_states.device
-        if seqlen < MIN_TILEMIX_SEQLEN:
+        over_cache, parent = int4_route(past_kv, self.layer_idx, attention_mask, seqlen)
+        if parent:
             return LlamaAttention.forward(self, hidden_states, position_embeddings=position_embeddings,
                                           attention_mask=attention_mask, past_key_values=past_kv,
                                           cache_position=cache_position, **kwargs)
         head_dim = self.config.hidden_size // self.config.num_attention_heads
-        cfg, block_n_mask, pmap = self._routing_for(seqlen, device)
+        if not over_cache:
+            cfg, block_n_mask, pmap = self._routing_for(seqlen, device)
 
         q = self.q_proj(hidden_states).view(bsz, seqlen, self.nh, head_dim).transpose(1, 2)
         k = self.k_proj(hidden_states).view(bsz, seqlen, self.nkv, head_dim).transpose(1, 2)
@@ -73,6 +76,9 @@ class TileMixLlamaAttention(TileMixRoutingMixin, LlamaAttention):
             cos, sin = position_embeddings
         cos, sin = cos.to(device), sin.to(device)
         q, k = self.apply_rotary(q, k, cos, sin)
+        if over_cache:
+            past_kv.append(k, v, self.layer_idx)
+            return self.o_proj(past_kv.attend(q, self.layer_idx, head_dim ** -0.5).reshape(bsz, seqlen, -1)), None
         if past_kv is not None:
             k, v = past_kv.update(k, v, self.layer_idx,
                                   cache_kwargs={"sin": sin, "cos": cos, "cache_position": cache_position})

@@ -16,7 +16,7 @@ from torch import Tensor
 from transformers.models.qwen2.modeling_qwen2 import Qwen2Attention
 
 from ..attention.tilemix_varlen import tilemix_varlen_attention
-from ._common import MIN_TILEMIX_SEQLEN, TileMixRoutingMixin, apply_rotary
+from ._common import TileMixRoutingMixin, apply_rotary, int4_route
 from .tilemix_llama import _swap_attention
 
 __all__ = ["TileMixqwenAttention", "inject_tilemix_into_qwen", "configure_tilemix_attention_pattern",
@@ -66,17 +66,19 @@ class TileMixqwenAttention(TileMixRoutingMixin, Qwen2Attention):
         bsz, seqlen, _ = hidden_states.size()
         hidden_states = self._ensure_cuda(hidden_states)
         device = hidden_states.device
-        if seqlen < MIN_TILEMIX_SEQLEN:
+        over_cache, parent = int4_route(past_key_values, self.layer_idx, attention_mask, seqlen)
+        if parent:
             return Qwen2Attention.forward(self, hidden_states, position_embeddings=position_embeddings,
                                           attention_mask=attention_mask, past_key_values=past_key_values,
                                           cache_position=cache_position, **kwargs)
         head_dim = self.config.hidden_size // self.config.num_attention_heads
-        cfg, block_n_mask, pmap = self._routing_for(seqlen, device)
-        skey = (seqlen, cfg.block_m, block_n_mask, pmap.data_ptr())
-        clean = self._sanitized.get(skey)
-        if clean is None:
-            clean = sanitize_precision_map(pmap, seqlen, block_n_mask)
-            self._sanitized[skey] = clean
+        if not over_cache:
+            cfg, block_n_mask, pmap = self._routing_for(seqlen, device)
+            skey = (seqlen, cfg.block_m, block_n_mask, pmap.data_ptr())
+            clean = self._sanitized.get(skey)
+            if clean is None:
+                clean = sanitize_precision_map(pmap, seqlen, block_n_mask)
+                self._sanitized[skey] = clean
 
         q = self.q_proj(hidden_states).view(bsz, seqlen, self.nh, head_dim).transpose(1, 2)
         k = self.k_proj(hidden_states).view(bsz, seqlen, self.nkv, head_dim).transpose(1, 2)
@@ -87,6 +89,10 @@ class TileMixqwenAttention(TileMixRoutingMixin, Qwen2Attention):
             cos, sin = self.rotary_emb(q, kwargs.get("position_ids"))
         cos, sin = cos.to(device), sin.to(device)
         q, k = apply_rotary(q, k, cos, sin)
+        if over_cache:
+            past_key_values.append(k, v, self.layer_idx)
+            out = past_key_values.attend(q, self.layer_idx, head_dim ** -0.5)
+            return self.o_proj(out.reshape(bsz, seqlen, -1)), None
         if past_key_values is not None:
             k, v = past_key_values.update(k, v, self.layer_idx,
                                           cache_kwargs={"sin": sin, "cos": cos, "cache_position": cache_position})
