@@ -314,7 +314,8 @@ int tilemix_kv4_load(const tilemix_kv4_rows_params* p, void* stream);
  * j <= seq_lens[b] - nq + i, and all of them without.  Grouped heads: query head h reads KV head
  * h / (heads_q / heads_k).  out = softmax(sm_scale q k^T) v over the cache's values;
  * a query that sees no key gets zeros, rows of `out` behind the last query stay as they are.
- * At most max_seqlen_q queries and max_seqlen_k keys of a sequence are read.
+ * At most max_seqlen_q queries and max_seqlen_k keys of a sequence are read, and no more keys
+ * than its table row has places for (2^30 at most); seq_lens[b] counts as that many.
  * `workspace`: tilemix_kv4_attn_workspace(p) bytes (0: may be NULL), 16-byte aligned, written
  * and read by this call alone.
  */

@@ -519,6 +519,69 @@ def test_infinite_and_large_queries():
     c.check()
 
 
+def test_small_weights_of_many_keys_count():
+    """One key 18 above 40000 others: together they weigh 0.06% (2^-26 each, below what fp16 holds beside a weight
+    of one); V is 0 at the one and 1 at the others, so that the output is their share.  Held 2^7 times larger they
+    are 2^-19, of fp16's steps of 2^-24: off by 2^-6 at most, beside the output's own rounding."""
+    dim, page, n = 64, 64, 40001
+    pages = -(-n // page)
+    pool = [np.zeros((pages, 1, page, 32), np.uint8), np.zeros((pages, 1, page, 2, 2), np.float16)] * 2
+    pool = [a.copy() for a in pool]
+    pool[1][0, 0, 0, 0, 1] = 18.0 / 32  # K: 18 / 32 in group 0 of key 0
+    pool[3][..., 1] = 1.0
+    pool[3][0, 0, 0, :, 1] = 0.0
+    table = np.arange(pages, dtype=np.int32)[None]
+    for tokens, group in ((1, 1), (1, 20), (130, 4)):
+        q = np.ones((tokens, group, dim))
+        got = paged_int4_attention(dev(q, torch.float16), to_cache(pool, dim), dev(table), ints([n]), ints([0, tokens]),
+                                   tokens, n, sm_scale=1.0)
+        seen = n - tokens + np.arange(tokens)  # of the others
+        want = (seen / (seen + np.exp(18.0)))[:, None, None]
+        assert (np.abs(got.double().cpu().numpy() - want) <= (2.0 ** -6 + 2.0 ** -11) * want).all()
+
+
+def test_offsets_past_32_bits():
+    """A pool whose codes take more than 4 GiB: the same rows in its first and its last pages."""
+    dim, heads, page = 128, 8, 64
+    pages = (1 << 32) // (heads * page * 64) + 40
+    cache = PagedInt4Cache.empty(pages, heads, dim, page)
+    assert cache.k_codes.numel() > 1 << 32
+    gen = torch.Generator().manual_seed(0)
+    lens = [900, 130]
+    k, v = (torch.randn(sum(lens), heads, dim, generator=gen).half().cuda() for _ in range(2))
+    cu = [0, 900, 1030]
+    results = []
+    for new in ([1, 1], [300, 2], [900, 130]):
+        q = torch.randn(sum(new), 24, dim, generator=gen).half().cuda()
+        for base in (0, pages - 20):
+            table = torch.full((2, 15), -1, dtype=torch.int32)
+            table[0], table[1, :3] = torch.arange(base, base + 15), torch.arange(base + 15, base + 18)
+            slots = torch.cat([table[b, torch.arange(n) // page].long() * page + torch.arange(n) % page
+                               for b, n in enumerate(lens)])
+            store_int4(k, v, cache, slots.cuda())
+            out = paged_int4_attention(q, cache, table.cuda(), ints(lens), ints([0, new[0], sum(new)]), max(new), 900)
+            results.append((out, *load_int4(cache, table.cuda(), ints(cu), 1030)))
+    for low, high in zip(results[::2], results[1::2]):
+        assert all(torch.equal(a, b) for a, b in zip(low, high))
+
+
+def test_lengths_past_the_table_and_offsets_out_of_range():
+    """seq_lens of more than a row's places, negative ones, cu_seqlens that start or end out of range."""
+    c = Call([100, 64], [3, 2], 4, 2, 64, seed=31)
+    q, cache, table, lens, cu, max_q, _ = c.device_args()
+    want = paged_int4_attention(q, cache, table[:, :4], ints([64, 64]), cu, max_q, 64)
+    got = paged_int4_attention(q, cache, table[:, :4], ints([10 ** 9, 64]), cu, max_q, 10 ** 9)
+    assert torch.equal(got, want)
+    out = torch.full_like(q, 5.0)
+    paged_int4_attention(q, cache, table, ints([-5, 64]), cu, max_q, 100, out=out)
+    assert not out[:3].any() and torch.equal(out[3:], want[3:])
+    for bad in ([-2 ** 31, 2, 5], [0, 2 ** 31 - 1, 5], [7, 3, 1], [0, -9, 2 ** 31 - 1]):
+        out.fill_(5.0)
+        paged_int4_attention(q, cache, table, lens, ints(bad), max_q, 100, out=out)
+        load_int4(cache, table, ints(bad), 9)
+    torch.cuda.synchronize()
+
+
 def test_the_same_page_in_several_sequences():
     """A shared prefix: table rows that name the same pages."""
     c = Call([100, 100, 64], [1, 1, 2], 4, 2, 64, seed=10)

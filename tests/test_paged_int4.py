@@ -241,7 +241,8 @@ def test_c_entry_points_refuse(lib):
 
     for change in (dict(heads_q=5), dict(heads_q=0), dict(batch=-1), dict(batch=65536), dict(max_seqlen_q=-1),
                    dict(max_seqlen_k=-1), dict(tokens_q=-1), dict(tokens_q=1 << 31), dict(table_columns=-1),
-                   dict(head_dim=200), dict(max_seqlen_q=2 ** 31 - 1)):
+                   dict(head_dim=200), dict(max_seqlen_q=2 ** 31 - 1),
+                   dict(table_columns=2 ** 27, max_seqlen_k=2 ** 30 + 1)):
         assert lib.tilemix_kv4_attn(ctypes.byref(attn(**change)), None) == 1, change
         assert lib.tilemix_kv4_attn_workspace(ctypes.byref(attn(**change))) == -1
     for change in (dict(q=None), dict(out=None), dict(seq_lens=None), dict(block_table=None)):

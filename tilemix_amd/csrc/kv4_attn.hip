@@ -7,9 +7,9 @@
 //
 // The mathematics of a tile, in fp32 but for the operands of the matrix instructions:
 //   S^T = K Q^T          keys x rows, K's values fp16(n s + m) exactly as the cache defines them
-//   p = exp2(S^T c - M)  c = sm_scale log2(e), M the row's running maximum
+//   p = exp2(S^T c - M)  c = sm_scale log2(e), M the row's running maximum less 7
 //   O^T += V^T P^T       channels x rows
-// p is rounded to fp16 for the second product (p <= 2^8, see kKv4Slack; relative error 2^-11,
+// p is rounded to fp16 for the second product (p <= 2^15, see kKv4Slack and kWeightUp; relative error 2^-11,
 // as small as the output's own rounding), and the row sum adds the same rounded weights.
 #include "kv4_common.h"
 
@@ -25,6 +25,10 @@ constexpr int kChunkRT = 2, kChunkRows = kWaves * 16 * kChunkRT;  // query rows 
 // The running maximum is raised when a row exceeds it by this much (in powers of two): most
 // tiles then leave the outputs unscaled.
 constexpr float kKv4Slack = 8.0f;
+// Weights are held 2^7 times too large, at most 2^15: then only those below 2^-32 of the largest vanish in fp16,
+// and 131072 of them weigh less than its last place (from 2^-25 on 0.4% of a sum could be lost behind one
+// large score).  Sums and outputs carry the same factor, which their quotient drops.
+constexpr float kWeightUp = 7.0f;
 constexpr float kNoKey = -1e30f;  // running maximum of a row without keys
 
 struct Kv4Args {
@@ -336,8 +340,8 @@ __device__ __forceinline__ void tile_weights(const f32x4 (&acc)[4], float scale,
   for (int w = 0; w < 2; ++w)
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      pf[w][2 * e] = (f16)__builtin_amdgcn_exp2f(__builtin_fmaf(acc[2 * w][e], scale, -top));
-      pf[w][2 * e + 1] = (f16)__builtin_amdgcn_exp2f(__builtin_fmaf(acc[2 * w + 1][e], scale, -top));
+      pf[w][2 * e] = (f16)__builtin_amdgcn_exp2f(__builtin_fmaf(acc[2 * w][e], scale, kWeightUp - top));
+      pf[w][2 * e + 1] = (f16)__builtin_amdgcn_exp2f(__builtin_fmaf(acc[2 * w + 1][e], scale, kWeightUp - top));
     }
 }
 // The row sums of the weights, on the matrix pipe: sixteen rows of ones (each result row is the sum).
@@ -985,6 +989,8 @@ __global__ void __launch_bounds__(256) kv4_join_kernel(const Kv4Args a, int bloc
   store_out(a.out, (it.start + token) * a.so_t + (it.h * a.group + head) * a.so_h + c, o, a.d - c, a.o_vec, a.bf);
 }
 
+constexpr int64_t kMostKeys = 1 << 30;  // of a sequence: places of keys ahead of the last one still fit 32 bits
+
 struct Plan {
   int block_rows, row_blocks, splits, split_tiles;
   int64_t bytes;
@@ -1023,7 +1029,8 @@ bool make_plan(const char* what, const tilemix_kv4_attn_params& p, Plan& plan) {
                    p.dtype))
     return false;
   if (p.heads_q <= 0 || p.heads_q % p.heads_k != 0 || p.batch < 0 || p.batch > 65535 || p.table_columns < 0 ||
-      p.max_seqlen_q < 0 || p.max_seqlen_k < 0 || p.tokens_q < 0 || p.tokens_q > INT32_MAX) {
+      p.max_seqlen_q < 0 || p.max_seqlen_k < 0 || p.tokens_q < 0 || p.tokens_q > INT32_MAX ||
+      std::min<int64_t>(p.max_seqlen_k, (int64_t)p.table_columns * p.page_size) > kMostKeys) {
     set_error("%s: invalid sizes (heads %d/%d, batch %d, table_columns %d, max_seqlen %d/%d, %lld queries)", what,
               p.heads_q, p.heads_k, p.batch, p.table_columns, p.max_seqlen_q, p.max_seqlen_k, (long long)p.tokens_q);
     return false;

@@ -236,7 +236,7 @@ __global__ void __launch_bounds__(256) kv4_load_kernel(const RowsArgs a) {
     const int64_t t = t0 + k * S::kRows;
     while (b + 1 < a.batch && a.cu[b + 1] <= t) ++b;
     row[k] = -1;
-    if (t < a.tokens && t >= a.cu[b] && t < a.cu[b + 1]) {
+    if (t < a.tokens && a.cu[b] >= 0 && t >= a.cu[b] && t < a.cu[b + 1]) {
       const int at = (int)t - a.cu[b], column = fast_div(at, a.by_page);
       const int page = column < a.columns ? a.table[b * a.s_table + column] : -1;
       if (page >= 0 && page < a.pages) row[k] = ((int64_t)page * a.heads + h) * a.by_page.d + at - column * a.by_page.d;
