@@ -450,6 +450,22 @@ def test_out_strides_and_rows_behind():
     assert torch.equal(paged_int4_attention(split, *rest), paged_int4_attention(split.contiguous(), *rest))
 
 
+@pytest.mark.parametrize("lens,new,heads,kv_heads", [([90, 40], [2, 1], 4, 2), ([5000], [1], 4, 2), ([300, 290], [300, 129], 6, 2),
+                                                     ([900], [70], 4, 1)])
+def test_out_may_be_q(lens, new, heads, kv_heads):
+    c = Call(lens, new, heads, kv_heads, 64, seed=8)
+    q, *rest = c.device_args()
+    want = paged_int4_attention(q, *rest)
+    assert torch.equal(paged_int4_attention(q, *rest, out=q), want) and not want.isnan().any()
+
+
+def test_out_may_be_q_of_a_chunk():
+    c = Call(seed=3, **CHUNKS["one"])
+    q, *rest = c.device_args()
+    want = paged_int4_attention(q, *rest)
+    assert torch.equal(paged_int4_attention(q, *rest, out=q), want) and not want.isnan().any()
+
+
 def test_bad_pages_are_not_seen():
     """Table entries out of range, in the middle and for a whole sequence."""
     c = Call([200, 100, 60], [1, 2, 1], 4, 2, 64, seed=4)

@@ -142,6 +142,26 @@ def test_attention_refuses():
                                  args.pop("cu_seqlens_q"), args.pop("max_seqlen_q"), args.pop("max_seqlen_k"), **args)
 
 
+def test_attention_refuses_rows_that_overlap_and_endless_scales():
+    c, table, lens = cache(), torch.zeros(5, 3, dtype=torch.int32), ints(8, 9, 1, 2, 3)
+    room = half(9, 6, 64)
+    q = room[2:7]
+    flat = half(5 * 6 * 64 + 64)
+    for match, changed in (
+            ("rows that lie apart", dict(out=flat.as_strided((5, 6, 64), (6 * 64, 63, 1)))),
+            ("rows that lie apart", dict(out=flat.as_strided((5, 6, 64), (5 * 64, 64, 1)))),
+            ("rows that lie apart", dict(out=flat.as_strided((5, 6, 64), (64, 4 * 64, 1)))),
+            ("q itself or have memory of its own", dict(out=room[1:6])),
+            ("sm_scale must be finite", dict(sm_scale=float("nan"))),
+            ("sm_scale must be finite", dict(sm_scale=1e39)),
+            ("sm_scale must be finite", dict(sm_scale=-float("inf")))):
+        with pytest.raises(ValueError, match=match):
+            paged_int4_attention(q, c, table, lens, None, 1, 9, **changed)
+    for out in (q, room[:5].clone(), half(6, 5, 64).transpose(0, 1), half(5, 6, 80)[..., 8:72]):
+        with pytest.raises(RuntimeError, match="GPU"):
+            paged_int4_attention(q, c, table, lens, None, 1, 9, out=out)
+
+
 def test_tables_refuse():
     t = PageTables.empty(9, 2, 4, 16, device="cpu")
     assert t.free_pages.tolist() == list(range(8, -1, -1)) and t.free_count.tolist() == [9]

@@ -155,6 +155,6 @@ def paged_int4_attention(q: Tensor, cache: PagedInt4Cache, block_table: Tensor, 
     ``h // (query heads // KV heads)``.  A query that sees no key gets zeros; keys of a page that the
     table does not name are not seen.  ``max_seqlen_q`` and ``max_seqlen_k`` (and the places of a table
     row) bound the queries and keys of a sequence: a longer one counts as that long.  Rows behind the
-    last query are left as they were in ``out`` (undefined without one)."""
+    last query are left as they were in ``out`` (undefined without one), which may be q itself."""
     return _native.host().kv4_attention(*cache._args, q, block_table, seq_lens, cu_seqlens_q, max_seqlen_q,
                                         max_seqlen_k, causal, sm_scale, out)

@@ -138,6 +138,14 @@ void check_vector(const at::Tensor& t, at::ScalarType dtype, const char* name, i
                     size < 0 ? std::string() : " of " + std::to_string(size), ", got ", t.sizes());
 }
 
+// Whether the rows [n0][n1] of t [n0, n1, d] lie apart (token-major or head-major, with any gaps).
+bool rows_apart(const at::Tensor& t) {
+  const int64_t n0 = t.size(0), n1 = t.size(1), d = t.size(2);
+  const int64_t s0 = n0 > 1 ? t.stride(0) : INT64_MAX, s1 = n1 > 1 ? t.stride(1) : INT64_MAX;
+  const int64_t low = std::min(s0, s1), high = std::max(s0, s1), n = s0 < s1 ? n0 : n1;
+  return (d <= 1 || t.stride(2) == 1) && low >= d && (high == INT64_MAX || high >= (n - 1) * low + d);
+}
+
 at::Tensor unit_stride(const at::Tensor& t) {
   return t.dim() == 0 || t.size(-1) <= 1 || t.stride(-1) == 1 ? t : t.contiguous();
 }
@@ -324,12 +332,14 @@ PyObject* kv4_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     scale = PyFloat_AsDouble(a[12]);
     if (scale == -1.0 && PyErr_Occurred()) throw python_error();
   }
+  TORCH_CHECK_VALUE(std::isfinite(static_cast<float>(scale)), "sm_scale must be finite in 32 bits, got ", scale);
   p.sm_scale = static_cast<float>(scale);
   if (out0 != nullptr) {
     check_dtype(*out0, q0.scalar_type(), "out");
-    TORCH_CHECK_VALUE(out0->sizes() == q0.sizes() && (c.head_dim == 1 || out0->stride(2) == 1) &&
-                          at::has_internal_overlap(*out0) != at::MemOverlap::Yes,
-                      "out must have q's shape ", q0.sizes(), ", contiguous rows and memory of its own");
+    TORCH_CHECK_VALUE(out0->sizes() == q0.sizes() && rows_apart(*out0), "out must have q's shape ", q0.sizes(),
+                      " and contiguous rows that lie apart, got ", out0->sizes(), " with strides ", out0->strides());
+    TORCH_CHECK_VALUE(at::get_overlap_status(*out0, q0) != at::MemOverlapStatus::Partial,
+                      "out must be q itself or have memory of its own");
   }
   check_device(c.device(), {&q0, &table0, &lens0, cu0, out0});
   const c10::DeviceGuard guard(c.device());
