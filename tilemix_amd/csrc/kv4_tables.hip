@@ -75,8 +75,12 @@ __device__ __forceinline__ int find(const int32_t* first, int n, int x) {
   return lo;
 }
 
+// The load of `value` has come back.
+__device__ __forceinline__ void arrived(int value) { asm volatile("" ::"v"(value)); }
+
 // True in all threads of the workgroup that comes here last: seq_lens, free_count and the new lengths have been
-// read by all then (their values are in LDS).  Nothing that the others wrote is read, so the count need not order it.
+// read by all then (before the barriers that every workgroup has passed: the lengths are in LDS, the count has arrived
+// in each wave).  Nothing that the others wrote is read, so the count need not order it.
 __device__ __forceinline__ bool last_workgroup(const TablesArgs& a) {
   __shared__ int last;
   if (gridDim.x == 1) return true;
@@ -113,6 +117,7 @@ __global__ void __launch_bounds__(kThreads) kv4_extend_kernel(const TablesArgs a
     base[r] = change;
     mine = __builtin_elementwise_add_sat(mine, (uint32_t)max(change, 0));
   }
+  arrived(count);
   const uint32_t tokens_before = scan_before(mine, sums[0]);
   uint32_t at = tokens_before, pages = 0;
   for (int r = r0; r < r1; ++r) {
@@ -210,6 +215,7 @@ __global__ void __launch_bounds__(kThreads) kv4_truncate_kernel(const TablesArgs
     base[r] = fast_div(held + page - 1, a.by_page) - fast_div(kept + page - 1, a.by_page);
     mine = __builtin_elementwise_add_sat(mine, (uint32_t)base[r]);
   }
+  arrived(count);
   uint32_t first = scan_before(mine, sums);
   for (int r = r0; r < r1; ++r) {
     const int back = base[r];
