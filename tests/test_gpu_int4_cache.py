@@ -170,3 +170,18 @@ def test_generate_crop_and_reset():
         assert own.get_seq_length() == 0 and int(own.tables.free_count) == own.layers[0].pool.pages
         first = model(prompt, past_key_values=own).logits[:, -1]
         assert torch.equal(first.argmax(-1), text[:, 50])
+
+
+def test_a_capture_is_refused():
+    """The cache counts on the host; after the refusal it goes on as if the call had not been."""
+    cache = Int4KVCache(1, 2, 64, 2, 64, page_size=16)
+    k = torch.randn(2, 2, 3, 64, device="cuda", dtype=torch.float16)
+    cache.append(k, k, 0)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(RuntimeError, match="no part in a graph capture"):
+            cache.append(k, k, 0)
+    assert cache.length == 3
+    cache.append(k, k, 0)
+    assert cache.length == 6 and cache.tables.seq_lens.tolist() == [6, 6]

@@ -72,3 +72,9 @@ def test_route():
 
 def test_module_is_exported_where_the_modules_are():
     assert TL.int4_route is int4_route
+
+
+@pytest.mark.parametrize("name", ["layers", "batch", "max_tokens", "page_size"])
+def test_sizes_of_nothing_are_refused(name):
+    with pytest.raises(ValueError, match="at least 1"):
+        make(**{name: 0})

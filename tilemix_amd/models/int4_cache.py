@@ -71,6 +71,9 @@ class Int4KVCache(Cache):
 
     def __init__(self, layers: int, kv_heads: int, head_dim: int, batch: int, max_tokens: int, *, page_size: int = 64,
                  device="cuda", unpadded: bool = False):
+        if min(layers, batch, max_tokens, page_size) < 1:
+            raise ValueError(f"Int4KVCache needs layers, sequences, tokens and a page size of at least 1, got {layers}, "
+                             f"{batch}, {max_tokens}, {page_size}")
         columns = -(-max_tokens // page_size)
         pools = (PagedInt4Cache.empty(batch * columns, kv_heads, head_dim, page_size, device) for _ in range(layers))
         super().__init__(layers=[_Int4Layer(self, pool, idx) for idx, pool in enumerate(pools)])
@@ -98,6 +101,10 @@ class Int4KVCache(Cache):
         if batch != self.batch:
             raise ValueError(f"Int4KVCache holds {self.batch} sequences, got {batch}")
         if layer.seen == self.length:
+            if key_states.is_cuda and torch.cuda.is_current_stream_capturing():
+                # The lengths that bound the kernels' work are kept here: a replay would go on with the captured ones.
+                raise RuntimeError("Int4KVCache counts its tokens on the host and takes no part in a graph capture; "
+                                   "PageTables and paged_int4_attention do")
             if self.length + new > self.max_tokens:
                 raise ValueError(f"Int4KVCache has room for {self.max_tokens} tokens a sequence, "
                                  f"got {self.length} and {new} more")
