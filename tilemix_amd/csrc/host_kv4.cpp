@@ -433,11 +433,21 @@ PyObject* kv4_extend(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const int64_t tokens = integer(a[7], "num_tokens", 0, INT32_MAX);
   const at::Device device = tables(a, p, lens, tokens);
   const c10::DeviceGuard guard(device);
-  const auto options = at::TensorOptions().device(device);
-  at::Tensor out[4] = {at::empty({tokens}, options.dtype(at::kLong)), at::empty({tokens}, options.dtype(at::kLong)),
-                       p.batch > 0 ? at::empty({p.batch + 1}, options.dtype(at::kInt))
-                                   : at::zeros({1}, options.dtype(at::kInt)),
-                       at::empty({p.batch}, options.dtype(at::kInt))};
+  // One allocation for the four: they are small, live as long as each other, and a second one takes the host a
+  // microsecond (a step of 64 sequences, extend and truncate: host 10.7 us with four, 9.2 with one).
+  const int64_t length[4] = {tokens, tokens, p.batch + 1, p.batch};
+  int64_t from[5] = {0};
+  for (int i = 0; i < 4; ++i) from[i + 1] = from[i] + (length[i] * (i < 2 ? 8 : 4) + 15) / 16 * 16;
+  const auto options = at::TensorOptions().device(device).dtype(at::kByte);
+  const at::Tensor room = p.batch > 0 ? at::empty({from[4]}, options) : at::zeros({from[4]}, options);
+  at::Tensor out[4];
+  for (int i = 0; i < 4; ++i) {
+    const auto dtype = c10::scalarTypeToTypeMeta(i < 2 ? at::kLong : at::kInt);
+    out[i] = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(room.storage()), room.key_set(), dtype);
+    c10::TensorImpl* const impl = out[i].unsafeGetTensorImpl();
+    impl->set_storage_offset(from[i] / (i < 2 ? 8 : 4));
+    impl->set_sizes_contiguous(c10::IntArrayRef(length[i]));
+  }
   p.lens = static_cast<const int32_t*>(lens.const_data_ptr());
   p.slots = static_cast<int64_t*>(out[0].data_ptr());
   p.positions = static_cast<int64_t*>(out[1].data_ptr());
