@@ -345,6 +345,68 @@ def test_chunk_kernel(name):
     assert np.isfinite(diff).all() and (diff <= tol).all(), f"worst {np.max(diff / tol):.2f} of the tolerance"
 
 
+def lengths(n, high, seed, low=0):
+    return [int(x) for x in np.random.default_rng(seed).integers(low, high + 1, n)]
+
+
+RAGGED = {  # batches whose keys are shared out by the sequences' lengths, more than 64 of them among those
+    "decode": dict(lens=lengths(150, 2500, 1), new=[1] * 150, heads=4, kv_heads=2, dim=64, page=32),
+    "decode_with_idle": dict(lens=lengths(70, 3000, 2), new=lengths(70, 1, 3), heads=3, kv_heads=3, dim=128, page=64),
+    "one_long": dict(lens=[30000] + lengths(9, 90, 4), new=[1] * 10, heads=6, kv_heads=2, dim=96, page=16, dtype="bf16"),
+    "nothing_but_one": dict(lens=[0] * 40 + [5000] + [0] * 40, new=[1] * 81, heads=2, kv_heads=1, dim=64, page=64),
+    "drafts": dict(lens=lengths(66, 2400, 5), new=lengths(66, 9, 6), heads=8, kv_heads=2, dim=64, page=16),
+    "drafts_few": dict(lens=[6100, 17, 0, 1500, 3300], new=[6, 6, 0, 6, 1], heads=24, kv_heads=8, dim=128, page=64),
+    "drafts_33": dict(lens=lengths(20, 4000, 7, 33), new=[33] * 20, heads=4, kv_heads=4, dim=32, page=48),
+    "see_all": dict(lens=lengths(12, 4000, 8), new=lengths(12, 12, 9), heads=8, kv_heads=4, dim=128, page=64, causal=False),
+    "chunks": dict(lens=lengths(70, 2900, 10, 300), new=[300] + lengths(69, 3, 11), heads=2, kv_heads=1, dim=64, page=64),
+    "chunks_few": dict(lens=[9000, 300, 4000], new=[200, 300, 50], heads=24, kv_heads=8, dim=128, page=64),
+}
+
+
+@pytest.mark.parametrize("name", RAGGED)
+def test_ragged_batches(name):
+    c = Call(seed=len(name), **RAGGED[name])
+    got = c.run()
+    ref, tol = want_on_gpu(c)
+    diff = np.abs(got.double().cpu().numpy() - ref)
+    assert np.isfinite(diff).all() and (diff <= tol).all(), f"worst {np.max(diff / tol):.2f} of the tolerance"
+    assert torch.equal(c.run(), got)
+
+
+def test_ragged_batch_in_a_graph_follows_the_lengths():
+    """Lengths that change between the replays: the pieces are found anew."""
+    c = Call(lengths(40, 3000, 12, 1), [1] * 40, 4, 2, 64, page=32, seed=12)
+    q, cache, table, lens, cu, max_q, max_k = c.device_args()
+    run = lambda: paged_int4_attention(q, cache, table, lens, cu, max_q, max_k)
+    run()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run()
+    for seed in range(4):
+        c.lens = [min(a, b) for a, b in zip(c.lens, lengths(40, 3000 >> seed, 20 + seed, 1))]
+        lens.copy_(ints(c.lens))
+        graph.replay()
+        torch.cuda.synchronize()
+        c.check(out)
+        assert torch.equal(run(), out)
+
+
+@pytest.mark.parametrize("new,heads", [(1, 4), (6, 8), (300, 2)])
+def test_queries_out_of_order_stay_inside(new, heads):
+    """Starts of sequences that do not ascend: nobody else's memory is touched, and the next call is right."""
+    lens = lengths(40, 2900, 13, 1500)
+    c = Call(lens, [new] * 40, heads, 1, 64, page=64, seed=13)
+    q, cache, table, seq, cu, max_q, max_k = c.device_args()
+    room = torch.full((q.shape[0] + 8, heads, 64), 9.0, dtype=torch.float16, device="cuda")
+    for bad in (cu.flip(0), torch.where(torch.arange(41, device="cuda") % 2 == 0, cu * 0, cu), cu * 0 - 5, cu * 0 + 2 ** 30):
+        paged_int4_attention(q, cache, table, seq, bad.int().contiguous(), max_q, max_k, out=room[4:-4])
+        assert (room[:4] == 9.0).all() and (room[-4:] == 9.0).all()
+    got = c.run()
+    ref, tol = want_on_gpu(c)
+    assert (np.abs(got.double().cpu().numpy() - ref) <= tol).all()
+
+
 def test_chunk_kernel_pages_nan_and_what_lies_behind():
     """Bad pages, stale rows behind the end and a stored NaN, with operands shared by the workgroup."""
     c = Call([3000, 700], [1000, 40], 6, 2, 128, page=16, seed=21)

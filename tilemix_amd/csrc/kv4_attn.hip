@@ -1,9 +1,9 @@
 // Attention over the paged 4-bit cache (format and arguments: include/tilemix_hip.h).
 //
 // A workgroup takes one (sequence, KV head), up to 16 RT of its query rows -- a row is a (query token,
-// query head of the group) pair -- and one split of the keys.  Its four waves take the split's
+// query head of the group) pair -- and one piece of the keys.  Its four waves take the piece's
 // 64-key tiles in turn and join their running maxima, sums and outputs in LDS at the end; with
-// several splits the parts go to the workspace and kv4_join_kernel adds them up.
+// several pieces the parts go to the workspace and kv4_join_kernel adds them up.
 //
 // The mathematics of a tile, in fp32 but for the operands of the matrix instructions:
 //   S^T = K Q^T          keys x rows, K's values fp16(n s + m) exactly as the cache defines them
@@ -21,7 +21,7 @@ namespace {
 
 constexpr int kTile = 64;  // keys
 constexpr int kWaves = 4;
-constexpr int kChunkRT = 2, kChunkRows = kWaves * 16 * kChunkRT;  // query rows of a wave (in 16s), of a workgroup
+constexpr int kChunkRT = 2, kChunkShift = 7, kChunkRows = kWaves * 16 * kChunkRT;  // query rows of a wave (in 16s), of a workgroup
 // The running maximum is raised when a row exceeds it by this much (in powers of two): most
 // tiles then leave the outputs unscaled.
 constexpr float kKv4Slack = 8.0f;
@@ -41,47 +41,176 @@ struct Kv4Args {
   const int32_t* table;
   const int32_t* lens;
   const int32_t* cu;
-  float* part;     // [item][split][row][channel] sums, unnormalised
-  float2* part_ml; // [item][split][row] maximum, sum
+  float* part;     // [head][unit][row][channel] sums, unnormalised
+  float2* part_ml; // [head][unit][row] maximum, sum
+  int2* notes;     // [sequence] number of its first workgroup, pieces
   int64_t sq_t, sq_h, so_t, so_h, s_table, tokens;
   float scale;
   int pages, hq, hk, group, d, columns, max_q, max_k, causal, bf, q_vec, o_vec;
-  int row_blocks, splits, split_tiles;
-  FastDiv by_page, by_group, by_splits;
+  int batch, block_shift, row_blocks;  // rows of a block: 1 << block_shift; blocks of max_q
+  int units, least, fit;               // workgroups of a head; see Kv4Splits
+  int each;                            // tiles of a piece of an even split
+  FastDiv by_page, by_group, by_heads, by_blocks, by_pieces, by_share, by_units;
 };
 
-// One (sequence, KV head, block of query rows): its rows and keys.
-struct Kv4Item {
-  int b, h, rb;
-  int64_t start;  // first query token
-  int nq, rows;   // queries, rows of all its blocks
-  int len;        // keys
-  int limit0;     // keys that query 0 sees (may be <= 0)
-  int kmax;       // keys that the block's last row sees
-};
+// How a call's keys are split: not at all (an item is one workgroup's), into the same number of tiles everywhere, or
+// by the sequences' lengths.
+enum Kv4Split { kNoSplit, kEvenSplit, kBalancedSplit };
 
-__device__ __forceinline__ Kv4Item kv4_item(const Kv4Args& a, int b, int h, int rb, int block_rows) {
-  Kv4Item it;
-  it.b = b;
-  it.h = h;
-  it.rb = rb;
+// The queries and keys of a sequence.
+struct Kv4Seq {
+  int start, nq, len;
+};
+__device__ __forceinline__ Kv4Seq kv4_seq(const Kv4Args& a, int b) {
   int64_t start = (int64_t)b * a.max_q;
   int nq = a.max_q;
   if (a.cu != nullptr) {
     start = a.cu[b];
     nq = a.cu[b + 1] - (int)start;
   }
-  if (start < 0 || start > a.tokens) nq = 0;
-  nq = (int)min((int64_t)min(nq, a.max_q), a.tokens - start);
-  it.start = start;
-  it.nq = max(nq, 0);
-  it.rows = it.nq * a.group;
+  const bool inside = start >= 0 && start <= a.tokens;
   const int64_t room = min((int64_t)a.columns * a.by_page.d, (int64_t)a.max_k);
-  it.len = (int)min((int64_t)max(a.lens[b], 0), room);
+  Kv4Seq s;
+  s.start = inside ? (int)start : 0;
+  s.nq = inside ? max((int)min((int64_t)min(nq, a.max_q), a.tokens - start), 0) : 0;
+  s.len = (int)min((int64_t)max(a.lens[b], 0), room);
+  return s;
+}
+
+// One (sequence, KV head, block of query rows): its rows and keys.
+struct Kv4Item : Kv4Seq {
+  int b, h, rb;
+  int rows;    // of all blocks
+  int limit0;  // keys that query 0 sees (may be <= 0)
+  int kmax;    // keys that the block's last row sees
+};
+__device__ __forceinline__ Kv4Item kv4_item(const Kv4Args& a, const Kv4Seq& seq, int b, int h, int rb) {
+  Kv4Item it;
+  static_cast<Kv4Seq&>(it) = seq;
+  it.b = b;
+  it.h = h;
+  it.rb = rb;
+  it.rows = it.nq * a.group;
   it.limit0 = a.causal ? it.len - it.nq + 1 : it.len;
-  const int last = min(it.rows, (rb + 1) * block_rows) - 1;
+  const int last = min(it.rows, (rb + 1) << a.block_shift) - 1;
   it.kmax = a.causal ? it.limit0 + fast_div(max(last, 0), a.by_group) : it.len;
   return it;
+}
+
+// ---- the keys of a call over the workgroups -----------------------------------------
+// How long the sequences of a batch are is known on the device only.  Every wave adds them up (64 at a time, one a
+// lane): `share` workgroups a head are to have the same work, `least` units of it at least; a sequence's blocks
+// of rows are split into as many pieces as that gives, of one size.  The pieces of all sequences are
+// numbered [sequence][block][piece]: a workgroup finds its own in the sums, about 1 us later than from its
+// index alone.  That costs batches of one length 0 to 2 us and saves the others the wait for their longest
+// sequence: calls in us, pieces of one size for all sequences / by their lengths (head_dim 128):
+//   decode, 24/8 heads, 48 of 200 .. 6000 57.6 / 51.5; 24 of 700 .. 9001 (28/4 heads) 29.1 / 26.4; 16 x 2048 (32/8)
+//   17.9 / 19.5; 32 x 4096 37.9 / 37.6;
+//   8 queries, 16 of 500 .. 6000 43.9 / 35.5, 8 x 4000 22.8 / 24.4; 40 of 300 .. 2500 (6 queries, 24/4) 41.3 / 33.0;
+//   256 queries, 4 of 600 .. 6000 122 / 77; 40 .. 100 queries, 8 of 500 .. 4000 87 / 49.
+__device__ __forceinline__ int kv4_blocks(const Kv4Args& a, const Kv4Seq& s) {
+  return (int)(((int64_t)s.nq * a.group + (1 << a.block_shift) - 1) >> a.block_shift);
+}
+__device__ __forceinline__ uint32_t kv4_tiles(int keys) { return keys <= 0 ? 0 : ((uint32_t)keys + kTile - 1) / kTile; }
+
+// The units: rounds of the four waves, or pairs of tiles that they go through together.
+__device__ __forceinline__ int kv4_work(const Kv4Args& a, int keys) {
+  const int shift = a.block_shift == kChunkShift ? 1 : 2;
+  return ((int)kv4_tiles(keys) + (1 << shift) - 1) >> shift;
+}
+
+struct Kv4Splits {
+  int unit;     // work of a piece
+  Kv4Seq mine;  // of the lane's sequence, among the 64 at hand
+
+  __device__ __forceinline__ Kv4Seq load(const Kv4Args& a, int c0) const {
+    const int b = c0 + (threadIdx.x & 63);
+    Kv4Seq s{};
+    if (b < a.batch) s = kv4_seq(a, b);
+    return s;
+  }
+  __device__ __forceinline__ explicit Kv4Splits(const Kv4Args& a) {
+    uint32_t total = 0;
+    for (int c0 = (a.batch - 1) & ~63; c0 >= 0; c0 -= 64) {
+      mine = load(a, c0);
+      const uint32_t work = (uint32_t)kv4_blocks(a, mine) * (uint32_t)kv4_work(a, mine.len);
+      total += (uint32_t)__builtin_amdgcn_readlane((int)wave_scan(work), 63);
+    }
+    // (below 2^31: fewer than 512 blocks of rows, of 2^22 units at most)
+    unit = max(fast_div((int)total + a.by_share.d - 1, a.by_share), a.least);
+    // Larger until the pieces are no more than the card takes at once, if that is asked for: with one more than
+    // that on a CU all wait for it (8 queries, 8 of 500 .. 6000: 25.8 us, 29.9 without this).
+    while (a.fit > 0 && unit < a.fit) {
+      int all = 0;
+      for (int c0 = (a.batch - 1) & ~63; c0 >= 0; c0 -= 64) {
+        if (a.batch > 64) mine = load(a, c0);
+        all += __builtin_amdgcn_readlane((int)wave_scan((uint32_t)(pieces(a) * kv4_blocks(a, mine))), 63);
+      }
+      if (all <= a.by_share.d) break;
+      unit += unit / 8 + 1;
+    }
+  }
+  // ceil(work / unit) = 1 + floor((work - 1/2) / unit), never more (the grid has no room for it): the factor is
+  // below 1 by more than the quotient's rounding, and by less than what is left of 1/2 up to 2^19 units.
+  __device__ __forceinline__ int pieces(const Kv4Args& a) const {
+    const float work = (float)kv4_work(a, mine.len) - 0.5f;  // exact
+    return 1 + (int)fmaxf(work * ((1.0f - 0x1p-20f) * __builtin_amdgcn_rcpf((float)unit)), 0.0f);
+  }
+};
+
+// Where a workgroup stands: a piece of one (sequence, block of rows).
+struct Kv4Place {
+  Kv4Seq seq;
+  int b, rb, split, pieces, in;  // in: number in the sequence
+};
+__device__ __forceinline__ Kv4Seq read_lane(const Kv4Seq& s, int lane) {
+  return Kv4Seq{__builtin_amdgcn_readlane(s.start, lane), __builtin_amdgcn_readlane(s.nq, lane),
+                __builtin_amdgcn_readlane(s.len, lane)};
+}
+// Of workgroup `unit` of a head; b = -1: there is none.
+template <Kv4Split kSplit>
+__device__ __forceinline__ Kv4Place kv4_place(const Kv4Args& a, int unit) {
+  if constexpr (kSplit != kBalancedSplit) {
+    Kv4Place at{};
+    const int item = fast_div(unit, a.by_pieces);
+    at.pieces = a.by_pieces.d;
+    at.split = unit - item * at.pieces;
+    at.b = fast_div(item, a.by_blocks);
+    at.rb = item - at.b * a.row_blocks;
+    return at;
+  }
+  Kv4Splits s(a);
+  Kv4Place at{};
+  at.b = -1;
+  for (int c0 = 0; c0 < a.batch; c0 += 64) {
+    if (c0 > 0) s.mine = s.load(a, c0);
+    const int pieces = s.pieces(a), blocks = kv4_blocks(a, s.mine), mine = pieces * blocks;
+    const int behind = (int)wave_scan((uint32_t)mine), all = __builtin_amdgcn_readlane(behind, 63);
+    if (unit < all) {
+      const int lane = __popcll(__ballot(behind <= unit));
+      at.in = unit - __builtin_amdgcn_readlane(behind - mine, lane);
+      const int n = __builtin_amdgcn_readlane(blocks, lane);
+      at.seq = read_lane(s.mine, lane);
+      at.pieces = __builtin_amdgcn_readlane(pieces, lane);
+      at.b = c0 + lane;
+      // (blocks: of the longest sequence, a sequence with one has no quotient to wait for)
+      at.rb = a.row_blocks > 1 ? (int)((uint32_t)at.in / (uint32_t)at.pieces) : 0;
+      at.split = at.in - at.rb * at.pieces;
+      return at;
+    }
+    unit -= all;
+  }
+  return at;
+}
+// Tiles of a piece; kWhole: whole rounds of the waves.
+template <bool kWhole>
+__device__ __forceinline__ int piece_tiles(const Kv4Seq& s, int pieces) {
+  const int tiles = (int)kv4_tiles(s.len), work = kWhole ? (tiles + 3) / 4 : tiles;  // at most 2^24
+  int each = (int)((float)work * __builtin_amdgcn_rcpf((float)pieces));  // (off by one)
+  each += each * pieces < work ? 1 : 0;
+  each += each * pieces < work ? 1 : 0;
+  each = max(each, 1);
+  return kWhole ? 4 * each : each;
 }
 
 __device__ __forceinline__ float lanes16_max(float x) {
@@ -422,28 +551,41 @@ struct ValueParams {
   }
 };
 
-template <int NG, int RT>
+template <int NG, int RT, Kv4Split kSplit>
 __global__ void __launch_bounds__(kWaves * 64, RT == 1 ? 3 : 2) kv4_attn_kernel(const Kv4Args a) {
   using Tile = Kv4Tile<NG>;
   constexpr int kCT = 2 * NG;  // tiles of 16 channels
   extern __shared__ __attribute__((aligned(16))) unsigned char smem[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15,
             g = lane >> 4;
-  const int rb = fast_div(blockIdx.x, a.by_splits), split = blockIdx.x - rb * a.splits;
-  const int first = split * a.split_tiles;
-  const Kv4Item it = kv4_item(a, blockIdx.z, blockIdx.y, rb, 16 * RT);
-  const int row0 = rb * 16 * RT;
-  if (row0 >= it.rows) return;
-  const int tiles = it.kmax <= 0 ? 0 : (it.kmax + kTile - 1) / kTile;
-  const int last = min(tiles, first + a.split_tiles);
-  if (first >= last && split > 0) return;
-
+  // KV heads are the fastest (kv4_chunk_kernel), but for one sequence's pieces, which are alike: 1 x 131072 37.5 us
+  // with the heads slowest, 38.2 with them fastest.
+  const int slow = fast_div(blockIdx.x, kSplit == kEvenSplit ? a.by_units : a.by_heads);
+  const int fast = blockIdx.x - slow * (kSplit == kEvenSplit ? a.units : a.hk);
+  const int unit = kSplit == kEvenSplit ? fast : slow, h = kSplit == kEvenSplit ? slow : fast;
+  const Kv4Place at = kv4_place<kSplit>(a, unit);
+  if (at.b < 0) return;
+  if (kSplit == kBalancedSplit && at.in == 0 && h == 0 && threadIdx.x == 0) a.notes[at.b] = make_int2(unit, at.pieces);
   // the first keys' places are on their way while the queries come
+  int first = kSplit == kEvenSplit ? at.split * a.each : 0, each = a.each;
+  if (kSplit == kBalancedSplit) {
+    each = piece_tiles<true>(at.seq, at.pieces);
+    first = at.split * each;
+  }
   Kv4Walk walk;
-  walk.table = a.table + it.b * a.s_table;
+  walk.table = a.table + at.b * a.s_table;
   walk.key0 = (first + wave) * kTile;
-  walk.end = min(it.kmax, last * kTile);
   walk.fetch(a, 0);
+  const Kv4Item it = kv4_item(a, kSplit == kBalancedSplit ? at.seq : kv4_seq(a, at.b), at.b, h, at.rb);
+  const int rb = at.rb, row0 = rb * 16 * RT;
+  if (row0 >= it.rows) return;
+  const bool joined = kSplit != kNoSplit && at.pieces > 1;
+  int last = kv4_tiles(it.kmax);
+  if (joined) {
+    last = min(last, first + each);
+    if (first >= last && at.split > 0) return;
+  }
+  walk.end = min(it.kmax, last * kTile);
   f16x8 qf[RT][NG];
   float scale[RT];
   int limit[RT];
@@ -579,7 +721,7 @@ __global__ void __launch_bounds__(kWaves * 64, RT == 1 ? 3 : 2) kv4_attn_kernel(
   for (int rt = 0; rt < RT; ++rt) {
     if (g == 0) lds_ml[(wave * RT + rt) * 16 + i] = make_float2(top[rt], sum[rt][0]);
   }
-  const int item = ((it.b * a.hk + it.h) * a.row_blocks + rb) * a.splits + split;
+  const int64_t part0 = ((int64_t)h * a.units + unit) * (16 * RT);
   f32x4* const lds_o = reinterpret_cast<f32x4*>(smem);
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
@@ -599,16 +741,16 @@ __global__ void __launch_bounds__(kWaves * 64, RT == 1 ? 3 : 2) kv4_attn_kernel(
     __syncthreads();
     const int row = row0 + 16 * rt + i, token = fast_div(row, a.by_group), head = row - token * a.group;
     if (row < it.rows) {
-      if (a.splits > 1 && wave == 0 && g == 0)
-        a.part_ml[(int64_t)item * (16 * RT) + 16 * rt + i] = make_float2(all_top, all_sum);
+      if (joined && wave == 0 && g == 0)
+        a.part_ml[part0 + 16 * rt + i] = make_float2(all_top, all_sum);
       const float norm = all_sum == 0.0f ? 0.0f : 1.0f / all_sum;
       for (int ct = wave; ct < kCT; ct += kWaves) {
         f32x4 r = lds_o[ct * 64 + lane];
 #pragma unroll
         for (int w = 1; w < kWaves; ++w) r += lds_o[(w * kCT + ct) * 64 + lane];
         const int c = 16 * ct + 4 * g;
-        if (a.splits > 1) {
-          *reinterpret_cast<f32x4*>(a.part + ((int64_t)item * (16 * RT) + 16 * rt + i) * (32 * NG) + c) = r;
+        if (joined) {
+          *reinterpret_cast<f32x4*>(a.part + (part0 + 16 * rt + i) * (32 * NG) + c) = r;
           continue;
         }
         r *= norm;
@@ -651,23 +793,34 @@ __device__ __forceinline__ void interleave() {
   }
 }
 
-template <int NG, int RT>
+template <int NG, int RT, Kv4Split kSplit>
 __global__ void __launch_bounds__(kWaves * 64, 2) kv4_chunk_kernel(const Kv4Args a) {
   constexpr int kCT = 2 * NG, kNP = Kv4Tile<NG>::kNP, kRows = kWaves * 16 * RT;
   __shared__ __attribute__((aligned(16))) ChunkLds<NG> lds;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15,
             g = lane >> 4;
-  const int rb = fast_div(blockIdx.y, a.by_splits), split = blockIdx.y - rb * a.splits;
-  const int first = split * a.split_tiles;
+  const int unit = fast_div(blockIdx.x, a.by_heads), h = blockIdx.x - unit * a.hk;
+  const Kv4Place at = kv4_place<kSplit>(a, unit);
+  if (at.b < 0) return;
+  if (kSplit == kBalancedSplit && at.in == 0 && h == 0 && threadIdx.x == 0) a.notes[at.b] = make_int2(unit, at.pieces);
+  int first = kSplit == kEvenSplit ? at.split * a.each : 0, each = a.each;
+  if (kSplit == kBalancedSplit) {
+    each = piece_tiles<false>(at.seq, at.pieces);
+    first = at.split * each;
+  }
   // The rows of the pool of block `wave` of the tiles first + 64 c .. + 63, one in each lane (-1: no page).
-  const int32_t* const table = a.table + blockIdx.z * a.s_table;
+  const int32_t* const table = a.table + at.b * a.s_table;
   auto key_of = [&](int n) { return (first + n + lane) * kTile + 16 * wave; };
   int ids = table_entry(a, table, key_of(0)), rows = -1;
-  const Kv4Item it = kv4_item(a, blockIdx.z, blockIdx.x, rb, kRows);
+  const Kv4Item it = kv4_item(a, kSplit == kBalancedSplit ? at.seq : kv4_seq(a, at.b), at.b, h, at.rb);
+  const int rb = at.rb;
   if (rb * kRows >= it.rows) return;
-  const int tiles = it.kmax <= 0 ? 0 : (it.kmax + kTile - 1) / kTile;
-  const int last = min(tiles, first + a.split_tiles);
-  if (first >= last && split > 0) return;
+  const bool joined = kSplit != kNoSplit && at.pieces > 1;
+  int last = kv4_tiles(it.kmax);
+  if (joined) {
+    last = min(last, first + each);
+    if (first >= last && at.split > 0) return;
+  }
   const int end = min(it.kmax, last * kTile);  // keys
 
   const int row0 = rb * kRows + wave * 16 * RT;  // of the wave
@@ -918,19 +1071,20 @@ __global__ void __launch_bounds__(kWaves * 64, 2) kv4_chunk_kernel(const Kv4Args
 
   // ---- each wave has its rows for itself ----
   if (!rows_there) return;
-  const int64_t item = ((int64_t)(it.b * a.hk + it.h) * a.row_blocks + rb) * a.splits + split;
+  const int at_end = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0));  // the lane: none kept for here
+  const int i_end = at_end & 15, g_end = at_end >> 4;
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
     const float all = sum[rt][0];
-    const int row = row0 + 16 * rt + i, token = fast_div(row, a.by_group), head = row - token * a.group;
+    const int row = row0 + 16 * rt + i_end, token = fast_div(row, a.by_group), head = row - token * a.group;
     if (row >= it.rows) continue;
-    const int64_t part = item * kRows + wave * 16 * RT + 16 * rt + i;
-    if (a.splits > 1 && g == 0) a.part_ml[part] = make_float2(top[rt], all);
+    const int64_t part = ((int64_t)h * a.units + unit) * kRows + wave * 16 * RT + 16 * rt + i_end;
+    if (joined && g_end == 0) a.part_ml[part] = make_float2(top[rt], all);
     const float norm = all == 0.0f ? 0.0f : 1.0f / all;
 #pragma unroll
     for (int ct = 0; ct < kCT; ++ct) {
-      const int c = 16 * ct + 4 * g;
-      if (a.splits > 1) *reinterpret_cast<f32x4*>(a.part + part * (32 * NG) + c) = o[rt][ct];
+      const int c = 16 * ct + 4 * g_end;
+      if (joined) *reinterpret_cast<f32x4*>(a.part + part * (32 * NG) + c) = o[rt][ct];
       else
         store_out(a.out, (it.start + token) * a.so_t + (it.h * a.group + head) * a.so_h + c, o[rt][ct] * norm, a.d - c,
                   a.o_vec, a.bf);
@@ -941,23 +1095,33 @@ __global__ void __launch_bounds__(kWaves * 64, 2) kv4_chunk_kernel(const Kv4Args
 // Adds up the splits of a row.  One thread takes four channels of every `lanes`-th split and keeps
 // its own running maximum; the `lanes` threads of a row's channels meet in LDS.
 template <int NG>
-__global__ void __launch_bounds__(256) kv4_join_kernel(const Kv4Args a, int block_rows, int lanes, int rows) {
+__global__ void __launch_bounds__(256) kv4_join_kernel(const Kv4Args a, bool balanced, int lanes, int rows) {
   constexpr int kC = 8 * NG;
   __shared__ f32x4 lds_o[256];
   __shared__ float2 lds_ml[256];
   const int unit = threadIdx.x / kC, c = 4 * (threadIdx.x - unit * kC), r = unit / lanes, lane = unit - r * lanes;
-  const int groups = (block_rows + rows - 1) / rows, rb = blockIdx.x / groups;
+  const int block_rows = 1 << a.block_shift, groups = (block_rows + rows - 1) / rows, rb = blockIdx.x / groups;
   const int in_block = (blockIdx.x - rb * groups) * rows + r;
-  const Kv4Item it = kv4_item(a, blockIdx.z, blockIdx.y, rb, block_rows);
+  const Kv4Seq seq = kv4_seq(a, blockIdx.z);
+  int before = blockIdx.z * a.row_blocks * a.by_pieces.d, pieces = a.by_pieces.d;
+  if (balanced) {
+    // (written by a workgroup of the sequence; what stands there if none was launched, with a cu out of order, is
+    // bounded here)
+    const int2 note = a.notes[blockIdx.z];
+    before = note.x;
+    pieces = note.y;
+    if (pieces <= 1 || (uint64_t)(uint32_t)before + (uint64_t)rb * (uint32_t)pieces >= (uint64_t)a.units) return;  // (one piece: it wrote the output)
+  }
+  const Kv4Item it = kv4_item(a, seq, blockIdx.z, blockIdx.y, rb);
   const int row = rb * block_rows + in_block;
   const bool there = r < rows && in_block < block_rows && row < it.rows;
   f32x4 o = {};
   float2 ml = make_float2(kNoKey, 0.0f);
   if (there) {
-    const int tiles = it.kmax <= 0 ? 0 : (it.kmax + kTile - 1) / kTile;
-    const int parts = max(1, (tiles + a.split_tiles - 1) / a.split_tiles);
-    const int64_t first =
-        (int64_t)((it.b * a.hk + it.h) * a.row_blocks + rb) * a.splits * block_rows + in_block;
+    const int each = !balanced ? a.each : block_rows == kChunkRows ? piece_tiles<false>(it, pieces) : piece_tiles<true>(it, pieces);
+    // (no more than there are workgroups, whatever cu holds)
+    const int parts = min(max(1, ((int)kv4_tiles(it.kmax) + each - 1) / each), a.units - before - rb * pieces);
+    const int64_t first = ((int64_t)it.h * a.units + before + rb * pieces) * block_rows + in_block;
 #pragma unroll 4
     for (int s = lane; s < parts; s += lanes) {
       const int64_t at = first + (int64_t)s * block_rows;
@@ -992,37 +1156,11 @@ __global__ void __launch_bounds__(256) kv4_join_kernel(const Kv4Args a, int bloc
 constexpr int64_t kMostKeys = 1 << 30;  // of a sequence: places of keys ahead of the last one still fit 32 bits
 
 struct Plan {
-  int block_rows, row_blocks, splits, split_tiles;
+  Kv4Split split;
+  int block_shift, row_blocks, units, share, least, fit, each, pieces;
   int64_t bytes;
 };
 
-// Tiles of a split.  A split costs the join (a second launch, 4 us) and each workgroup's start and end (3 us, 10
-// with the chunk kernel, of which two fit a CU); too few leave the card waiting for the longest sequence.
-// Calls in us (head_dim 128, 24/8 heads unless said), this rule / others:
-//   * up to 12 tiles one: 1 x 700 (14/2 heads x 64) 8.2, split 9.5; 16 x 512 10.0 / 11.8;
-//   * few (sequence, head) pairs: two workgroups a CU.  1 x 131072 in 64 42.4, 48 45.7, 96 46.6; 3 of 2000 .. 30000
-//     in 21 30.1, 16 34.7, 32 31.1; 1 x 1024 in four 11.5, one 12.9;
-//   * else 16 tiles each (four a wave), as lengths differ and the longest sequence is waited for: 24 of 700 ..
-//     9001 (28/4 heads) in 9 29.6, 6 36.3; 24 of 61 .. 5000 in 5 29.4, 3 36.8; 16 of 61 .. 5000 in 5 25.6, 7
-//     26.1; 32 x 1024 in one 14.7, two 18.5;
-//   * but no more than three workgroups a CU, all that are resident: 64 x 8192 in one 126, two 131, four
-//     134; 48 of 200 .. 6000 in two 62.4, four 67.2; 32 x 4096 in three 42.8, four 44.2.
-int64_t plan_split(int64_t items, int64_t tiles, int block_rows) {
-  if (block_rows == kChunkRows) {
-    const int64_t splits = std::min(std::max<int64_t>(512 / items, 1), std::max<int64_t>(tiles / 8, 1));
-    return (tiles + splits - 1) / splits;
-  }
-  if (tiles <= 12) return tiles;
-  int64_t splits;
-  if (items < 64) {
-    splits = std::min(512 / items, tiles / 4);
-  } else {
-    splits = (tiles + 15) / 16;
-    if (items * splits >= 1024) splits = std::max<int64_t>(768 / items, 1);
-  }
-  const int64_t each = (tiles + splits - 1) / splits;
-  return (each + kWaves - 1) / kWaves * kWaves;  // the waves take whole tiles in turn
-}
 
 bool make_plan(const char* what, const tilemix_kv4_attn_params& p, Plan& plan) {
   if (!kv4_pool_ok(what, p.k_codes, p.k_params, p.v_codes, p.v_params, p.pages, p.page_size, p.heads_k, p.head_dim,
@@ -1035,7 +1173,7 @@ bool make_plan(const char* what, const tilemix_kv4_attn_params& p, Plan& plan) {
               p.heads_q, p.heads_k, p.batch, p.table_columns, p.max_seqlen_q, p.max_seqlen_k, (long long)p.tokens_q);
     return false;
   }
-  const int64_t rows = (int64_t)p.max_seqlen_q * (p.heads_q / p.heads_k);
+  const int64_t group = p.heads_q / p.heads_k, rows = (int64_t)p.max_seqlen_q * group;
   const int64_t keys = std::min<int64_t>(p.max_seqlen_k, (int64_t)p.table_columns * p.page_size);
   const int64_t tiles = std::max<int64_t>((keys + kTile - 1) / kTile, 1);
   // The chunk kernel needs rows to share its conversions among, and work that outweighs its start and end; the
@@ -1044,45 +1182,83 @@ bool make_plan(const char* what, const tilemix_kv4_attn_params& p, Plan& plan) {
   // 44.2, 1 x 40000 (20000) 49.5 / 47.0; 300 rows 1 x 4000 (5040) 28.4 / 31.4, 1 x 40000 (50000) 111 / 88.
   const int64_t blocks32 = (rows + 31) / 32;
   const bool few = blocks32 * p.heads_k * p.batch * tiles <= 10000;
-  plan.block_rows = rows <= 16 ? 16 : rows <= 96 || few ? 32 : kChunkRows;
-  const int64_t blocks = (rows + plan.block_rows - 1) / plan.block_rows;
-  const int64_t items = std::max<int64_t>(blocks * p.heads_k * p.batch, 1);
-  const int64_t split_tiles = plan_split(items, tiles, plan.block_rows);
-  const int64_t splits = (tiles + split_tiles - 1) / split_tiles;
-  const int64_t grid = blocks * splits;
-  if (rows > INT32_MAX / 2 || grid > (plan.block_rows < kChunkRows ? (1 << 24) - 1 : 65535) || items * splits > INT32_MAX / 64) {
+  const bool chunk = rows > 96 && !few;
+  plan.block_shift = rows <= 16 ? 4 : chunk ? kChunkShift : 5;
+  const int64_t block_rows = (int64_t)1 << plan.block_shift;
+  const int64_t blocks = (rows + block_rows - 1) / block_rows;  // of a sequence, at most
+  int64_t units = blocks * p.batch;                             // workgroups of a head
+  if (rows > INT32_MAX / 2 || units * p.heads_k >= 1 << 24) {
     set_error("%s: too many queries for one call (%lld rows a sequence, batch %d)", what, (long long)rows, p.batch);
     return false;
   }
+  plan.share = plan.least = plan.fit = plan.each = 0;
+  plan.pieces = 1;
+  plan.bytes = 0;
+  plan.split = kNoSplit;
+  const int64_t items = std::max<int64_t>(std::min(units, p.tokens_q * group / block_rows + p.batch) * p.heads_k, 1);
+  // A split costs the join (a second launch, 4 us) and each workgroup's start and end (3 us, 10 with the chunk
+  // kernel): none for short sequences or where the items fill the card.  Calls in us (24/8 heads x 128 unless
+  // said), whole / split: 1 x 700 (14/2 heads x 64) 8.2 / 9.5; 16 x 512 10.0 / 11.8; 8 x 1024 13.0 / 15.3; 32 x 1024
+  // 15.2 / 17.4; but 1 x 1024 12.9 / 11.5; 64 x 8192 126 / 131.
+  if (chunk ? items < 256 && tiles >= 16 : items < 512 && tiles > (items < 64 ? 12 : 16)) {
+    if (p.batch == 1) {
+      // Two workgroups a CU: 1 x 131072 in 64 pieces 42.4, 48 45.7, 96 46.6.
+      const int64_t whole = chunk ? 1 : kWaves;
+      const int64_t pieces = std::max<int64_t>(std::min(512 / items, tiles / (chunk ? 8 : 4)), 1);
+      plan.each = (int)(((tiles + pieces - 1) / pieces + whole - 1) / whole * whole);
+      plan.pieces = (int)((tiles + plan.each - 1) / plan.each);
+      plan.split = plan.pieces > 1 ? kEvenSplit : kNoSplit;
+      units *= plan.pieces;
+    } else {
+      plan.split = kBalancedSplit;
+      plan.share = (int)std::max<int64_t>((plan.block_shift == 5 && items <= 96 ? 256 : 512) / p.heads_k, 1);
+      // Blocks of 32 rows hold two workgroups a CU, and do best with one where that gives pieces short enough: 8 of
+      // 1500 .. 6144 (5 queries, 32/8 heads; 64 items) 26.1 with 256 workgroups, 30.4 with 512; 16 of 500 .. 6000 (8
+      // queries, 128 items) 42.9 / 35.5.  Those of 16 rows hold three: room for what is over.
+      if (plan.block_shift == 4) {
+        plan.least = items < 64 ? 1 : 4;
+        units = items / p.heads_k + plan.share;
+      } else {
+        plan.least = chunk ? 4 : 2;
+        plan.fit = (int)((tiles + 1) / 2);  // (no piece has more work)
+        units = std::max<int64_t>(items / p.heads_k, plan.share);
+      }
+      plan.pieces = (int)std::min<int64_t>(units * p.heads_k / items, (tiles + 3) / 4);  // on average
+    }
+  }
+  if (plan.split != kNoSplit) {
+    const int64_t width = (p.head_dim + kKv4Group - 1) / kKv4Group * kKv4Group;
+    plan.bytes = units * p.heads_k * block_rows * (width * 4 + 8) + p.batch * 8;
+  }
   plan.row_blocks = (int)blocks;
-  plan.splits = (int)splits;
-  plan.split_tiles = (int)split_tiles;
-  const int width = (p.head_dim + kKv4Group - 1) / kKv4Group * kKv4Group;
-  plan.bytes = splits > 1 ? items * splits * plan.block_rows * (width * 4 + 8) : 0;
+  plan.units = (int)units;
   return true;
 }
 
+template <int NG, Kv4Split kSplit>
+void launch_split(const Kv4Args& a, hipStream_t stream) {
+  // KV heads are the fastest: the workgroups of a head, which read the same keys, meet on few XCDs.
+  const dim3 grid((unsigned)a.units * a.hk), block(kWaves * 64);
+  constexpr int lds1 = kv4_lds_bytes<NG, 1>(), lds2 = kv4_lds_bytes<NG, 2>();
+  if (a.block_shift == 4) hipLaunchKernelGGL((kv4_attn_kernel<NG, 1, kSplit>), grid, block, lds1, stream, a);
+  else if (a.block_shift == 5) hipLaunchKernelGGL((kv4_attn_kernel<NG, 2, kSplit>), grid, block, lds2, stream, a);
+  else hipLaunchKernelGGL((kv4_chunk_kernel<NG, kChunkRT, kSplit>), grid, block, 0, stream, a);
+}
+
 template <int NG>
-void launch_kv4(const Kv4Args& a, int block_rows, int batch, hipStream_t stream) {
-  if (block_rows < kChunkRows) {
-    const dim3 grid((unsigned)(a.row_blocks * a.splits), a.hk, batch), block(kWaves * 64);
-    constexpr int lds1 = kv4_lds_bytes<NG, 1>(), lds2 = kv4_lds_bytes<NG, 2>();
-    if (block_rows == 16) hipLaunchKernelGGL((kv4_attn_kernel<NG, 1>), grid, block, lds1, stream, a);
-    else hipLaunchKernelGGL((kv4_attn_kernel<NG, 2>), grid, block, lds2, stream, a);
-  } else {
-    // Heads are the fastest: the workgroups of a head, which read the same keys, meet on few XCDs.
-    hipLaunchKernelGGL((kv4_chunk_kernel<NG, kChunkRT>), dim3(a.hk, (unsigned)(a.row_blocks * a.splits), batch),
-                       dim3(kWaves * 64), 0, stream, a);
-  }
-  if (a.splits > 1) {
-    // about four splits a thread
-    constexpr int units = 256 / (8 * NG);
-    int lanes = 1;
-    while (lanes * 2 <= units && lanes * 4 < a.splits) lanes *= 2;
-    const int rows = units / lanes;
-    const dim3 grid((unsigned)(a.row_blocks * ((block_rows + rows - 1) / rows)), a.hk, batch);
-    hipLaunchKernelGGL((kv4_join_kernel<NG>), grid, dim3(256), 0, stream, a, block_rows, lanes, rows);
-  }
+void launch_kv4(const Kv4Args& a, const Plan& plan, hipStream_t stream) {
+  if (plan.split == kNoSplit) launch_split<NG, kNoSplit>(a, stream);
+  else if (plan.split == kEvenSplit) launch_split<NG, kEvenSplit>(a, stream);
+  else launch_split<NG, kBalancedSplit>(a, stream);
+  if (plan.split == kNoSplit) return;
+  // about four pieces a thread
+  constexpr int units = 256 / (8 * NG);
+  const int block_rows = 1 << a.block_shift;
+  int lanes = 1;
+  while (lanes * 2 <= units && lanes * 4 < plan.pieces) lanes *= 2;
+  const int rows = units / lanes;
+  const dim3 grid((unsigned)(a.row_blocks * ((block_rows + rows - 1) / rows)), a.hk, a.batch);
+  hipLaunchKernelGGL((kv4_join_kernel<NG>), grid, dim3(256), 0, stream, a, plan.split == kBalancedSplit, lanes, rows);
 }
 
 }  // namespace
@@ -1120,8 +1296,11 @@ int launch_kv4_attn(const tilemix_kv4_attn_params& p, hipStream_t stream) {
   a.lens = p.seq_lens;
   a.cu = p.cu_seqlens_q;
   a.part = static_cast<float*>(p.workspace);
-  const int64_t parts = (int64_t)p.batch * p.heads_k * plan.row_blocks * plan.splits * plan.block_rows;
-  if (plan.bytes > 0) a.part_ml = reinterpret_cast<float2*>(a.part + parts * width);
+  if (plan.bytes > 0) {
+    const int64_t parts = ((int64_t)plan.units * p.heads_k) << plan.block_shift;
+    a.part_ml = reinterpret_cast<float2*>(a.part + parts * width);
+    a.notes = reinterpret_cast<int2*>(a.part_ml + parts);
+  }
   a.sq_t = p.stride_q_token;
   a.sq_h = p.stride_q_head;
   a.so_t = p.stride_o_token;
@@ -1141,24 +1320,32 @@ int launch_kv4_attn(const tilemix_kv4_attn_params& p, hipStream_t stream) {
   a.bf = p.dtype;
   a.q_vec = (reinterpret_cast<uintptr_t>(p.q) & 15) == 0 && ((p.stride_q_token | p.stride_q_head) & 7) == 0;
   a.o_vec = (reinterpret_cast<uintptr_t>(p.out) & 7) == 0 && ((p.stride_o_token | p.stride_o_head) & 3) == 0;
+  a.batch = p.batch;
+  a.block_shift = plan.block_shift;
   a.row_blocks = plan.row_blocks;
-  a.splits = plan.splits;
-  a.split_tiles = plan.split_tiles;
+  a.units = plan.units;
+  a.least = plan.least;
+  a.fit = plan.fit;
+  a.each = plan.each;
   a.by_page = make_fast_div(p.page_size);
   a.by_group = make_fast_div(a.group);
-  a.by_splits = make_fast_div(a.splits);
+  a.by_heads = make_fast_div(a.hk);
+  a.by_blocks = make_fast_div(a.row_blocks);
+  a.by_pieces = make_fast_div(plan.split == kEvenSplit ? plan.pieces : 1);
+  a.by_units = make_fast_div(a.units);
+  a.by_share = make_fast_div(std::max(plan.share, 1));
   switch (width / kKv4Group) {
     case 1:
-      launch_kv4<1>(a, plan.block_rows, p.batch, stream);
+      launch_kv4<1>(a, plan, stream);
       break;
     case 2:
-      launch_kv4<2>(a, plan.block_rows, p.batch, stream);
+      launch_kv4<2>(a, plan, stream);
       break;
     case 3:
-      launch_kv4<3>(a, plan.block_rows, p.batch, stream);
+      launch_kv4<3>(a, plan, stream);
       break;
     default:
-      launch_kv4<4>(a, plan.block_rows, p.batch, stream);
+      launch_kv4<4>(a, plan, stream);
   }
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) {

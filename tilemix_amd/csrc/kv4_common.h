@@ -35,6 +35,23 @@ __device__ __forceinline__ bool kv4_not_finite(uint32_t param) {
   return (param & 0x7c00u) == 0x7c00u || (param & 0x7c000000u) == 0x7c000000u;
 }
 
+// x + the values of the lanes before it in the wave (saturating, so that sums past 32 bits stay past every bound).
+// Shifts within 16 lanes, then the last lane of a row to the rows behind it.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t add_shifted(uint32_t x) {
+  return __builtin_elementwise_add_sat(
+      x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xf, false));
+}
+__device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
+  x = add_shifted<0x111, 0xf>(x);
+  x = add_shifted<0x112, 0xf>(x);
+  x = add_shifted<0x114, 0xf>(x);
+  x = add_shifted<0x118, 0xf>(x);
+  x = add_shifted<0x142, 0xa>(x);
+  x = add_shifted<0x143, 0xc>(x);
+  return x;
+}
+
 typedef __bf16 bf16;
 typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));

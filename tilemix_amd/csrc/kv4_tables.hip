@@ -33,23 +33,6 @@ struct TablesArgs {
   FastDiv by_page;
 };
 
-// x + the values of the lanes before it in the wave (saturating, so that sums past 32 bits stay past every bound).
-// Shifts within 16 lanes, then the last lane of a row to the rows behind it.
-template <int CTRL, int ROWS>
-__device__ __forceinline__ uint32_t add_shifted(uint32_t x) {
-  return __builtin_elementwise_add_sat(
-      x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xf, false));
-}
-__device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
-  x = add_shifted<0x111, 0xf>(x);
-  x = add_shifted<0x112, 0xf>(x);
-  x = add_shifted<0x114, 0xf>(x);
-  x = add_shifted<0x118, 0xf>(x);
-  x = add_shifted<0x142, 0xa>(x);
-  x = add_shifted<0x143, 0xc>(x);
-  return x;
-}
-
 // The sum over the workgroup's threads before this one; `sums`: a place of its own for every scan of a kernel.
 __device__ __forceinline__ uint32_t scan_before(uint32_t x, uint32_t* sums) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
