@@ -403,35 +403,41 @@ __device__ __forceinline__ void use_queries(const Kv4Args& a, const Kv4Item& it,
     limit[rt] = a.causal ? it.limit0 + fast_div(row0 + 16 * rt + i, a.by_group) : it.len;
     // A negative scale is the queries' sign; none is a product that leaves the maximum at zero.
     scale[rt] = fmaxf(fabsf(a.scale), 1e-37f);
-    f32x8 x[NG];
-    float top = 0.0f;
+    u32x4 w[NG];
 #pragma unroll
-    for (int s = 0; s < NG; ++s)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const uint32_t pair = raw[rt][s][e];  // (a bit cast of a vector's element would take the first one)
-        const f16x2 h = __builtin_bit_cast(f16x2, pair);
-        x[s][2 * e] = a.bf ? __uint_as_float(pair << 16) : (float)h[0];
-        x[s][2 * e + 1] = a.bf ? __uint_as_float(pair & 0xffff0000u) : (float)h[1];
-        top = fmaxf(top, fmaxf(fabsf(x[s][2 * e]), fabsf(x[s][2 * e + 1])));
-      }
+    for (int s = 0; s < NG; ++s) w[s] = raw[rt][s];
     // bf16 queries are held as fp16 times a power of two of their row: exact but for elements below
     // 2^-14 of the row's largest, which lose no more than 2^-25 of that one.
     if (a.bf) {
-      const int e = __builtin_amdgcn_frexp_expf(lanes16_max(top));
-      scale[rt] = ldexpf(scale[rt], e);
+      float top = 0.0f;
 #pragma unroll
       for (int s = 0; s < NG; ++s)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[s][j] = ldexpf(x[s][j], -e);
+        for (int e = 0; e < 4; ++e)
+          top = fmaxf(top, fmaxf(fabsf(__uint_as_float(w[s][e] << 16)), fabsf(__uint_as_float(w[s][e] & 0xffff0000u))));
+      const int e2 = __builtin_amdgcn_frexp_expf(lanes16_max(top));
+      scale[rt] = ldexpf(scale[rt], e2);
+#pragma unroll
+      for (int s = 0; s < NG; ++s)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const f16x2 h = {(f16)ldexpf(__uint_as_float(w[s][e] << 16), -e2),
+                           (f16)ldexpf(__uint_as_float(w[s][e] & 0xffff0000u), -e2)};
+          w[s][e] = __builtin_bit_cast(uint32_t, h);
+        }
     }
+    // in the pairs' order
+    const uint32_t sign = a.scale < 0.0f ? 0x80008000u : 0u;
 #pragma unroll
-    for (int s = 0; s < NG; ++s)
+    for (int s = 0; s < NG; ++s) {
+      u32x4 r;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        qf[rt][s][2 * j] = (f16)(a.scale < 0.0f ? -x[s][j] : x[s][j]);
-        qf[rt][s][2 * j + 1] = (f16)(a.scale < 0.0f ? -x[s][j + 4] : x[s][j + 4]);
+      for (int j = 0; j < 2; ++j) {
+        r[2 * j] = __builtin_amdgcn_perm(w[s][j + 2], w[s][j], 0x05040100u) ^ sign;
+        r[2 * j + 1] = __builtin_amdgcn_perm(w[s][j + 2], w[s][j], 0x07060302u) ^ sign;
       }
+      qf[rt][s] = __builtin_bit_cast(f16x8, r);
+    }
   }
 }
 
