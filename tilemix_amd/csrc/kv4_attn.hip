@@ -21,7 +21,9 @@ namespace {
 
 constexpr int kTile = 64;  // keys
 constexpr int kWaves = 4;
-constexpr int kChunkRT = 2, kChunkShift = 7, kChunkRows = kWaves * 16 * kChunkRT;  // query rows of a wave (in 16s), of a workgroup
+// The chunk kernel's query rows, of a wave in 16s and of a workgroup.
+constexpr int kChunkRT = 2, kChunkRows = kWaves * 16 * kChunkRT, kChunkShift = 7;
+static_assert(1 << kChunkShift == kChunkRows, "rows of a block are a power of two");
 // The running maximum is raised when a row exceeds it by this much (in powers of two): most
 // tiles then leave the outputs unscaled.
 constexpr float kKv4Slack = 8.0f;
@@ -111,12 +113,14 @@ __device__ __forceinline__ Kv4Item kv4_item(const Kv4Args& a, const Kv4Seq& seq,
 __device__ __forceinline__ int kv4_blocks(const Kv4Args& a, const Kv4Seq& s) {
   return (int)(((int64_t)s.nq * a.group + (1 << a.block_shift) - 1) >> a.block_shift);
 }
-__device__ __forceinline__ uint32_t kv4_tiles(int keys) { return keys <= 0 ? 0 : ((uint32_t)keys + kTile - 1) / kTile; }
+__device__ __forceinline__ int kv4_tiles(int keys) {
+  return keys <= 0 ? 0 : (int)(((uint32_t)keys + kTile - 1) / kTile);
+}
 
 // The units: rounds of the four waves, or pairs of tiles that they go through together.
 __device__ __forceinline__ int kv4_work(const Kv4Args& a, int keys) {
   const int shift = a.block_shift == kChunkShift ? 1 : 2;
-  return ((int)kv4_tiles(keys) + (1 << shift) - 1) >> shift;
+  return (kv4_tiles(keys) + (1 << shift) - 1) >> shift;
 }
 
 struct Kv4Splits {
@@ -169,7 +173,7 @@ __device__ __forceinline__ Kv4Seq read_lane(const Kv4Seq& s, int lane) {
 }
 // Of workgroup `unit` of a head; b = -1: there is none.
 template <Kv4Split kSplit>
-__device__ __forceinline__ Kv4Place kv4_place(const Kv4Args& a, int unit) {
+__device__ __forceinline__ Kv4Place kv4_place(const Kv4Args& a, int unit, int h) {
   if constexpr (kSplit != kBalancedSplit) {
     Kv4Place at{};
     const int item = fast_div(unit, a.by_pieces);
@@ -179,6 +183,7 @@ __device__ __forceinline__ Kv4Place kv4_place(const Kv4Args& a, int unit) {
     at.rb = item - at.b * a.row_blocks;
     return at;
   }
+  const int whole = unit;
   Kv4Splits s(a);
   Kv4Place at{};
   at.b = -1;
@@ -196,6 +201,7 @@ __device__ __forceinline__ Kv4Place kv4_place(const Kv4Args& a, int unit) {
       // (blocks: of the longest sequence, a sequence with one has no quotient to wait for)
       at.rb = a.row_blocks > 1 ? (int)((uint32_t)at.in / (uint32_t)at.pieces) : 0;
       at.split = at.in - at.rb * at.pieces;
+      if (at.in == 0 && h == 0 && threadIdx.x == 0) a.notes[at.b] = make_int2(whole, at.pieces);  // for the join
       return at;
     }
     unit -= all;
@@ -205,7 +211,7 @@ __device__ __forceinline__ Kv4Place kv4_place(const Kv4Args& a, int unit) {
 // Tiles of a piece; kWhole: whole rounds of the waves.
 template <bool kWhole>
 __device__ __forceinline__ int piece_tiles(const Kv4Seq& s, int pieces) {
-  const int tiles = (int)kv4_tiles(s.len), work = kWhole ? (tiles + 3) / 4 : tiles;  // at most 2^24
+  const int tiles = kv4_tiles(s.len), work = kWhole ? (tiles + 3) / 4 : tiles;  // at most 2^24
   int each = (int)((float)work * __builtin_amdgcn_rcpf((float)pieces));  // (off by one)
   each += each * pieces < work ? 1 : 0;
   each += each * pieces < work ? 1 : 0;
@@ -414,7 +420,8 @@ __device__ __forceinline__ void use_queries(const Kv4Args& a, const Kv4Item& it,
       for (int s = 0; s < NG; ++s)
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          top = fmaxf(top, fmaxf(fabsf(__uint_as_float(w[s][e] << 16)), fabsf(__uint_as_float(w[s][e] & 0xffff0000u))));
+          top = fmaxf(top, fmaxf(fabsf(__uint_as_float(w[s][e] << 16)),
+                                 fabsf(__uint_as_float(w[s][e] & 0xffff0000u))));
       const int e2 = __builtin_amdgcn_frexp_expf(lanes16_max(top));
       scale[rt] = ldexpf(scale[rt], e2);
 #pragma unroll
@@ -557,6 +564,11 @@ struct ValueParams {
   }
 };
 
+// Bound by HBM where the card is full (64 x 8192 keys, 24/8 heads x 128: 672 MB in 123 us, 5.4 TB/s; its vector
+// instructions, 600 a tile and wave of which the codes take 400, are 60% of that time), and for short or few sequences by
+// the chain of loads before the first tile (lengths, table, codes: about 5 us) and the tiles that a wave takes
+// one after the other.  Keys over the lanes and codes in registers leave LDS to V alone; waves take whole tiles
+// so that none waits for another before the end.
 template <int NG, int RT, Kv4Split kSplit>
 __global__ void __launch_bounds__(kWaves * 64, RT == 1 ? 3 : 2) kv4_attn_kernel(const Kv4Args a) {
   using Tile = Kv4Tile<NG>;
@@ -569,9 +581,8 @@ __global__ void __launch_bounds__(kWaves * 64, RT == 1 ? 3 : 2) kv4_attn_kernel(
   const int slow = fast_div(blockIdx.x, kSplit == kEvenSplit ? a.by_units : a.by_heads);
   const int fast = blockIdx.x - slow * (kSplit == kEvenSplit ? a.units : a.hk);
   const int unit = kSplit == kEvenSplit ? fast : slow, h = kSplit == kEvenSplit ? slow : fast;
-  const Kv4Place at = kv4_place<kSplit>(a, unit);
+  const Kv4Place at = kv4_place<kSplit>(a, unit, h);
   if (at.b < 0) return;
-  if (kSplit == kBalancedSplit && at.in == 0 && h == 0 && threadIdx.x == 0) a.notes[at.b] = make_int2(unit, at.pieces);
   // the first keys' places are on their way while the queries come
   int first = kSplit == kEvenSplit ? at.split * a.each : 0, each = a.each;
   if (kSplit == kBalancedSplit) {
@@ -776,6 +787,9 @@ __global__ void __launch_bounds__(kWaves * 64, RT == 1 ? 3 : 2) kv4_attn_kernel(
 // the values of tile n beside the conversion of K's tile n + 2 and V's tile n + 1; the codes after those are
 // on their way.  One barrier a tile.  K's codes come in registers (wave t: block t), V's as copies to
 // LDS, from which wave t makes the channels ct = t and t + 4.
+// With two workgroups a CU a tile of both takes 2.4 us (64000 keys: 815 TFLOP/s, 0.62 of a large GEMM's rate; the
+// matrix instructions alone would take 1.5, vector instructions are issued 46% of the time).  512 queries at 8000 keys
+// (24/8 heads x 128): 77 us, of which the conversion is 14, exp2 5, the start 10, the partial sums 5.
 template <int NG>
 struct ChunkLds {
   f16x8 k[2][4 * NG * 64];      // [tile][(t NG + s) 64 + lane]
@@ -806,9 +820,8 @@ __global__ void __launch_bounds__(kWaves * 64, 2) kv4_chunk_kernel(const Kv4Args
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), i = lane & 15,
             g = lane >> 4;
   const int unit = fast_div(blockIdx.x, a.by_heads), h = blockIdx.x - unit * a.hk;
-  const Kv4Place at = kv4_place<kSplit>(a, unit);
+  const Kv4Place at = kv4_place<kSplit>(a, unit, h);
   if (at.b < 0) return;
-  if (kSplit == kBalancedSplit && at.in == 0 && h == 0 && threadIdx.x == 0) a.notes[at.b] = make_int2(unit, at.pieces);
   int first = kSplit == kEvenSplit ? at.split * a.each : 0, each = a.each;
   if (kSplit == kBalancedSplit) {
     each = piece_tiles<false>(at.seq, at.pieces);
@@ -1077,7 +1090,7 @@ __global__ void __launch_bounds__(kWaves * 64, 2) kv4_chunk_kernel(const Kv4Args
 
   // ---- each wave has its rows for itself ----
   if (!rows_there) return;
-  const int at_end = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0));  // the lane: none kept for here
+  const int at_end = __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0));  // lane: no register holds it
   const int i_end = at_end & 15, g_end = at_end >> 4;
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
@@ -1116,7 +1129,8 @@ __global__ void __launch_bounds__(256) kv4_join_kernel(const Kv4Args a, bool bal
     const int2 note = a.notes[blockIdx.z];
     before = note.x;
     pieces = note.y;
-    if (pieces <= 1 || (uint64_t)(uint32_t)before + (uint64_t)rb * (uint32_t)pieces >= (uint64_t)a.units) return;  // (one piece: it wrote the output)
+    if (pieces <= 1) return;  // it wrote the output
+    if ((uint64_t)(uint32_t)before + (uint64_t)rb * (uint32_t)pieces >= (uint64_t)a.units) return;
   }
   const Kv4Item it = kv4_item(a, seq, blockIdx.z, blockIdx.y, rb);
   const int row = rb * block_rows + in_block;
@@ -1124,9 +1138,11 @@ __global__ void __launch_bounds__(256) kv4_join_kernel(const Kv4Args a, bool bal
   f32x4 o = {};
   float2 ml = make_float2(kNoKey, 0.0f);
   if (there) {
-    const int each = !balanced ? a.each : block_rows == kChunkRows ? piece_tiles<false>(it, pieces) : piece_tiles<true>(it, pieces);
+    const int each = !balanced                ? a.each
+                     : block_rows == kChunkRows ? piece_tiles<false>(it, pieces)
+                                                : piece_tiles<true>(it, pieces);
     // (no more than there are workgroups, whatever cu holds)
-    const int parts = min(max(1, ((int)kv4_tiles(it.kmax) + each - 1) / each), a.units - before - rb * pieces);
+    const int parts = min(max(1, (kv4_tiles(it.kmax) + each - 1) / each), a.units - before - rb * pieces);
     const int64_t first = ((int64_t)it.h * a.units + before + rb * pieces) * block_rows + in_block;
 #pragma unroll 4
     for (int s = lane; s < parts; s += lanes) {
