@@ -257,6 +257,47 @@ def test_store_rounding_of_every_quotient():
     assert np.array_equal(cache.v_params.reshape(tokens, 1, 4, 2).cpu().numpy(), params)
 
 
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+def test_store_ties_and_odd_groups_side_by_side(dtype):
+    """Exact halves between two codes go to the even one; ranges below fp16's normal numbers, constant groups, values
+    beyond the limit, infinities and NaN take their own way within a wave, in any company."""
+    rng = np.random.default_rng(11)
+    dim, page, tokens = 128, 16, 640
+    x = np.zeros((tokens, 2, 4, 32))
+    kind = rng.integers(0, 9, (tokens, 2, 4))
+    kind[:64], kind[64:128] = 0, 1  # (whole waves of ties)
+    for at in np.ndindex(*kind.shape):
+        n, k = rng.integers(0, 16, 32), kind[at]
+        n[:2] = 0, 15
+        if k in (0, 1):  # minimum, then halves: quotients k + 1/2 exactly
+            step = 2.0 ** rng.integers(-6, 3)
+            x[at] = (n + np.where((n < 15) & (n > 0), 0.5, 0.0)) * step - 8 * step * k
+        elif k == 2:  # a range of a few of fp16's smallest steps
+            x[at] = rng.integers(-9, 25, 32) * 2.0 ** -24
+        elif k == 3:
+            x[at] = rng.standard_normal()
+        elif k == 4:  # a minimum that fp16 does not have, a narrow range
+            x[at] = 1000.0 + rng.uniform(0, 8, 32)
+        elif k == 5:
+            x[at] = rng.choice([65408.0, 65472.0, 65504.0, -65504.0, 3.0], 32)
+        elif k == 6:
+            x[at] = np.where(rng.random(32) < 0.1, rng.choice([np.inf, -np.inf], 32), rng.standard_normal(32))
+        elif k == 7:
+            x[at] = np.where(rng.random(32) < 0.1, np.nan, rng.standard_normal(32))
+        else:
+            x[at] = rng.standard_normal(32)
+    x = rounded(x.reshape(tokens, 2, dim), dtype)
+    cache = PagedInt4Cache.empty(tokens // page, 2, dim, page)
+    t = dev(x, TYPES[dtype])
+    store_int4(t, t.flip(0), cache, torch.arange(tokens).cuda())
+    codes, params = P.quantise(x)
+    for got, want in ((cache.k_codes, codes), (cache.v_codes, codes[::-1])):
+        assert np.array_equal(got.transpose(1, 2).reshape(tokens, 2, -1).cpu().numpy(), want)
+    for got, want in ((cache.k_params, params), (cache.v_params, params[::-1])):
+        got = got.transpose(1, 2).reshape(tokens, 2, 4, 2).cpu().numpy()
+        assert np.array_equal(got, want.reshape(got.shape), equal_nan=True)
+
+
 def test_load_of_pages_that_are_not_there():
     """Table entries out of range and tokens past the table's columns read as zeros."""
     dim, page = 64, 16

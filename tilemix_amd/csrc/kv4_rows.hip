@@ -43,7 +43,8 @@ struct RowsArgs {
 // row, so that a wave reads whole rows in 16-byte pieces and the four lanes of a group find its range among
 // them.  A thread's loads are all in flight together, behind one look at the token's place.
 // 16384 tokens of 8 heads x 128, 88 MB each way: load 16.4 us (5.4 TB/s, a large copy's rate; K and V by threads of
-// their own 25), store 21.4 (4.1 TB/s, its 110 vector instructions a word take about 13 of it; IEEE divisions 33).
+// their own 25), store 17.4 (5.1 TB/s; bound by its vector instructions: 20.9 with every value clamped and the codes
+// shifted together in whole numbers, 33 with IEEE divisions).
 template <int NG>
 struct RowSplit {
   static constexpr int kWords = 4 * NG;
@@ -143,11 +144,61 @@ __device__ __forceinline__ float divide(float x, float y, float r) {
   return __builtin_fmaf(__builtin_fmaf(-q, y, x), r, q);
 }
 
-// The codes of a word of eight channels and, in every lane of the group, the group's parameters.
+// The codes of a word of eight channels and, in every lane of the group, the group's parameters.  kPlain: there is
+// neither a NaN nor anything beyond the limit among the wave's values.
+template <typename T, bool kPlain>
+__device__ __forceinline__ uint32_t quantise8(const u32x4& raw, bool present, bool nan, uint32_t& param) {
+  constexpr bool kHalf = std::is_same<T, f16>::value;
+  typename std::conditional<kHalf, Eight16, EightBf16>::type v(raw);
+  // (the four lanes of a group are in or out together; a word behind the last channel has no say)
+  float lo = present ? v.least() : __builtin_inff();
+  float hi = present ? v.most() : -__builtin_inff();
+  lo = fminf(lo, quad_xor1(lo));
+  hi = fmaxf(hi, quad_xor1(hi));
+  lo = fminf(lo, quad_xor2(lo));
+  hi = fmaxf(hi, quad_xor2(hi));
+  if (!kPlain) {
+    lo = __builtin_amdgcn_fmed3f(lo, -kKv4Limit, kKv4Limit);
+    hi = __builtin_amdgcn_fmed3f(hi, -kKv4Limit, kKv4Limit);
+    v.cap();
+  }
+  f16 s = (f16)keep32(divide(hi - lo, 15.0f, 1.0f / 15.0f)), m = (f16)lo;
+  if (!kPlain) {
+    float bad = nan && present ? 1.0f : 0.0f;
+    bad = fmaxf(bad, quad_xor1(bad));
+    bad = fmaxf(bad, quad_xor2(bad));
+    if (bad != 0.0f) {
+      s = (f16)0.0f;
+      m = (f16)__builtin_nanf("");
+    }
+  }
+  param = (uint32_t)__builtin_bit_cast(uint16_t, s) | (uint32_t)__builtin_bit_cast(uint16_t, m) << 16;
+  // 1 / s: a Newton step on the hardware reciprocal leaves 2^-22 of a last place before its rounding, and s has 11
+  // bits: 1 / s is no nearer than 2^-12 of a last place to where two roundings meet.  So it is the right one.
+  const float step = (float)s, least = (float)m, near = __builtin_amdgcn_rcpf(step);
+  const float recip = __builtin_fmaf(__builtin_fmaf(-step, near, 1.0f), near, near);
+  // A quotient becomes a byte, rounded to the nearest even number and 0 from below; even and odd channels make a word
+  // of bytes each.  It is 15.5 or more only where s lost bits of the range: below the normal numbers of
+  // fp16, or to a minimum that fp16 does not have.
+  uint32_t even = 0, odd = 0;
+  auto code = [&](int e, float q) {
+    uint32_t& to = e & 1 ? odd : even;
+    to = __builtin_amdgcn_cvt_pk_u8_f32(q, e >> 1, to);
+  };
+  if (kPlain && kHalf && __all(step >= 0x1p-14f || !present)) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) code(e, divide(v.less(e, least), step, recip));
+    return even | odd << 4;
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    code(e, __builtin_amdgcn_fmed3f(divide(v.less(e, least), step, recip), 0.0f, 15.0f));
+  return step > 0.0f ? even | odd << 4 : 0u;
+}
 template <typename T>
 __device__ __forceinline__ uint32_t quantise8(const u32x4& raw, bool present, uint32_t& param) {
-  typename std::conditional<std::is_same<T, f16>::value, Eight16, EightBf16>::type v(raw);
-  constexpr uint32_t kInf = std::is_same<T, f16>::value ? 0x7c00u : 0x7f80u;
+  constexpr bool kHalf = std::is_same<T, f16>::value;
+  constexpr uint32_t kInf = kHalf ? 0x7c00u : 0x7f80u, kMost = kHalf ? 0x7bfcu : 0x477fu;  // kKv4Limit or next below
   typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
   u16x2 size = {};
 #pragma unroll
@@ -155,44 +206,12 @@ __device__ __forceinline__ uint32_t quantise8(const u32x4& raw, bool present, ui
     const uint32_t pair = raw[e] & 0x7fff7fffu;
     size = __builtin_elementwise_max(size, __builtin_bit_cast(u16x2, pair));
   }
-  const bool nan = size[0] > kInf || size[1] > kInf;
-  // (the four lanes of a group are in or out together; a word behind the last channel has no say)
-  float lo = present ? v.least() : __builtin_inff();
-  float hi = present ? v.most() : -__builtin_inff();
-  float bad = nan && present ? 1.0f : 0.0f;
-  lo = fminf(lo, quad_xor1(lo));
-  hi = fmaxf(hi, quad_xor1(hi));
-  bad = fmaxf(bad, quad_xor1(bad));
-  lo = fminf(lo, quad_xor2(lo));
-  hi = fmaxf(hi, quad_xor2(hi));
-  bad = fmaxf(bad, quad_xor2(bad));
-  lo = __builtin_amdgcn_fmed3f(lo, -kKv4Limit, kKv4Limit);
-  hi = __builtin_amdgcn_fmed3f(hi, -kKv4Limit, kKv4Limit);
-  f16 s = (f16)keep32(divide(hi - lo, 15.0f, 1.0f / 15.0f)), m = (f16)lo;
-  if (bad != 0.0f) {
-    s = (f16)0.0f;
-    m = (f16)__builtin_nanf("");
-  }
-  param = (uint32_t)__builtin_bit_cast(uint16_t, s) | (uint32_t)__builtin_bit_cast(uint16_t, m) << 16;
-  // 1 / s: a Newton step on the hardware reciprocal leaves 2^-22 of a last place before its rounding, and s has 11
-  // bits: 1 / s is no nearer than 2^-12 of a last place to where two roundings meet.  So it is the right one.
-  // Adding 1.5 2^23 rounds to a whole number in the low bits; the sum of the shifted results counts that
-  // constant's bits once a code.  (Minus infinity makes a NaN here, which the median takes for the smallest: code 0.)
-  const float step = (float)s, least = (float)m, near = __builtin_amdgcn_rcpf(step);
-  const float recip = __builtin_fmaf(__builtin_fmaf(-step, near, 1.0f), near, near);
-  constexpr uint32_t kMagic = 0x4b400000u;
-  uint32_t word = 0u - (kMagic + (kMagic << 4) + (kMagic << 8) + (kMagic << 12) + (kMagic << 16) + (kMagic << 20) +
-                        (kMagic << 24) + (kMagic << 28));
-  v.cap();
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const float n = __builtin_amdgcn_fmed3f(divide(v.less(e, least), step, recip), 0.0f, 15.0f);
-    word += __builtin_bit_cast(uint32_t, n + 12582912.0f) << (4 * e);
-  }
-  return step > 0.0f ? word : 0u;
+  const uint32_t largest = max((uint32_t)size[0], (uint32_t)size[1]);
+  if (__all(largest <= kMost)) return quantise8<T, true>(raw, present, false, param);
+  return quantise8<T, false>(raw, present, largest > kInf, param);
 }
 
-// (One token a thread: two measured 21.6 us for 16384 tokens of 8 heads x 128, four 24.5, one 21.4.)
+// (One token a thread: 21.4 us where two took 21.6 and four 24.5, before the last two steps above.)
 template <int NG, typename T>
 __global__ void __launch_bounds__(256) kv4_store_kernel(const RowsArgs a) {
   using S = RowSplit<NG>;
