@@ -181,6 +181,9 @@ __device__ __forceinline__ Kv4Place kv4_place(const Kv4Args& a, int unit, int h)
     at.split = unit - item * at.pieces;
     at.b = fast_div(item, a.by_blocks);
     at.rb = item - at.b * a.row_blocks;
+    // The last blocks of rows, which see the most keys, go first (us, before / after: 8192 queries of 2 sequences, 24/8
+    // heads x 128, 978 / 882; 4096 of 8 1005 / 955; 1 .. 1030 of 6 over up to 4100 keys, 32/8, 223 / 210).
+    if (kSplit == kNoSplit) at.rb = a.row_blocks - 1 - at.rb;
     return at;
   }
   const int whole = unit;
