@@ -523,6 +523,13 @@ def test_bounds_on_queries_and_keys():
     assert (diff[keep] <= tol[keep]).all()
 
 
+@pytest.mark.parametrize("lens,new", [([900, 40], [3, 1]), ([6000, 2000, 2500], [40, 1, 90])])
+def test_loose_bounds_cost_nothing(lens, new):
+    """max_seqlen_q and max_seqlen_k far above what there is: the same values."""
+    c = Call(lens, new, 6, 2, 64, page=16, seed=31, max_q=2 ** 28, max_k=2 ** 31 - 1)
+    c.check()
+
+
 def test_empty_calls():
     c = Call([0, 0], [1, 2], 4, 2, 64)
     assert not c.run().any()

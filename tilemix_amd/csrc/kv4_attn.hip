@@ -141,14 +141,14 @@ struct Kv4Splits {
       total += (uint32_t)__builtin_amdgcn_readlane((int)wave_scan(work), 63);
     }
     // (below 2^31: fewer than 512 blocks of rows, of 2^22 units at most)
-    unit = max(fast_div((int)total + a.by_share.d - 1, a.by_share), a.least);
+    unit = max(fast_div((int)(total + (uint32_t)a.by_share.d - 1), a.by_share), a.least);
     // Larger until the pieces are no more than the card takes at once, if that is asked for: with one more than
     // that on a CU all wait for it (8 queries, 8 of 500 .. 6000: 25.8 us, 29.9 without this).
     while (a.fit > 0 && unit < a.fit) {
       int all = 0;
       for (int c0 = (a.batch - 1) & ~63; c0 >= 0; c0 -= 64) {
         if (a.batch > 64) mine = load(a, c0);
-        all += __builtin_amdgcn_readlane((int)wave_scan((uint32_t)(pieces(a) * kv4_blocks(a, mine))), 63);
+        all += __builtin_amdgcn_readlane((int)wave_scan((uint32_t)pieces(a) * (uint32_t)kv4_blocks(a, mine)), 63);
       }
       if (all <= a.by_share.d) break;
       unit += unit / 8 + 1;
@@ -192,12 +192,13 @@ __device__ __forceinline__ Kv4Place kv4_place(const Kv4Args& a, int unit, int h)
   at.b = -1;
   for (int c0 = 0; c0 < a.batch; c0 += 64) {
     if (c0 > 0) s.mine = s.load(a, c0);
-    const int pieces = s.pieces(a), blocks = kv4_blocks(a, s.mine), mine = pieces * blocks;
+    // (with a cu out of order the sums may pass 32 bits: then no workgroup finds itself here, and whichever does
+    // is within its sequence, as none is beyond it)
+    const int pieces = s.pieces(a), mine = (int)((uint32_t)pieces * (uint32_t)kv4_blocks(a, s.mine));
     const int behind = (int)wave_scan((uint32_t)mine), all = __builtin_amdgcn_readlane(behind, 63);
     if (unit < all) {
       const int lane = __popcll(__ballot(behind <= unit));
       at.in = unit - __builtin_amdgcn_readlane(behind - mine, lane);
-      const int n = __builtin_amdgcn_readlane(blocks, lane);
       at.seq = read_lane(s.mine, lane);
       at.pieces = __builtin_amdgcn_readlane(pieces, lane);
       at.b = c0 + lane;
@@ -1198,7 +1199,8 @@ bool make_plan(const char* what, const tilemix_kv4_attn_params& p, Plan& plan) {
               p.heads_q, p.heads_k, p.batch, p.table_columns, p.max_seqlen_q, p.max_seqlen_k, (long long)p.tokens_q);
     return false;
   }
-  const int64_t group = p.heads_q / p.heads_k, rows = (int64_t)p.max_seqlen_q * group;
+  // (rows of a sequence: no more than there are queries, however loose the bound)
+  const int64_t group = p.heads_q / p.heads_k, rows = std::min<int64_t>(p.max_seqlen_q, p.tokens_q) * group;
   const int64_t keys = std::min<int64_t>(p.max_seqlen_k, (int64_t)p.table_columns * p.page_size);
   const int64_t tiles = std::max<int64_t>((keys + kTile - 1) / kTile, 1);
   // The chunk kernel needs rows to share its conversions among, and work that outweighs its start and end; the
@@ -1212,8 +1214,9 @@ bool make_plan(const char* what, const tilemix_kv4_attn_params& p, Plan& plan) {
   const int64_t block_rows = (int64_t)1 << plan.block_shift;
   const int64_t blocks = (rows + block_rows - 1) / block_rows;  // of a sequence, at most
   int64_t units = blocks * p.batch;                             // workgroups of a head
-  if (rows > INT32_MAX / 2 || units * p.heads_k >= 1 << 24) {
-    set_error("%s: too many queries for one call (%lld rows a sequence, batch %d)", what, (long long)rows, p.batch);
+  if (p.max_seqlen_q * group > INT32_MAX / 2 || units * p.heads_k >= 1 << 24) {
+    set_error("%s: too many queries for one call (%lld rows a sequence, batch %d)", what,
+              (long long)(p.max_seqlen_q * group), p.batch);
     return false;
   }
   plan.share = plan.least = plan.fit = plan.each = 0;
