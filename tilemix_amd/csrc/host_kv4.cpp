@@ -150,6 +150,15 @@ at::Tensor unit_stride(const at::Tensor& t) {
   return t.dim() == 0 || t.size(-1) <= 1 || t.stride(-1) == 1 ? t : t.contiguous();
 }
 
+// A contiguous tensor of its own in the memory of another, `from` bytes in.
+at::Tensor part_of(const at::Tensor& room, at::ScalarType type, int64_t from, c10::IntArrayRef sizes) {
+  const auto dtype = c10::scalarTypeToTypeMeta(type);
+  at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(room.storage()), room.key_set(), dtype);
+  t.unsafeGetTensorImpl()->set_storage_offset(from / static_cast<int64_t>(dtype.itemsize()));
+  t.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
+  return t;
+}
+
 void* stream_of(at::Device device) { return c10::hip::getCurrentHIPStream(device.index()).stream(); }
 
 void check_status(int status) {
@@ -269,8 +278,20 @@ PyObject* kv4_load(PyObject*, PyObject* const* a, Py_ssize_t n) {
   check_device(c.device(), {&table0, &cu0});
   const c10::DeviceGuard guard(c.device());
   const at::Tensor table = unit_stride(table0), cu = unit_stride(cu0);
-  const auto options = at::TensorOptions().device(c.device()).dtype(dtype);
-  at::Tensor k = at::empty({p.tokens, c.heads, c.head_dim}, options), v = at::empty_like(k);
+  // Short sequences: one allocation for both (the host's time for the call 0.6 us less).  Large ones may be freed
+  // one by one.
+  const auto options = at::TensorOptions().device(c.device());
+  const int64_t sizes[3] = {p.tokens, c.heads, c.head_dim};
+  const int64_t bytes = (p.tokens * c.heads * c.head_dim * 2 + 15) / 16 * 16;
+  at::Tensor k, v;
+  if (bytes <= 1 << 20) {
+    const at::Tensor room = at::empty({2 * bytes}, options.dtype(at::kByte));
+    k = part_of(room, dtype, 0, sizes);
+    v = part_of(room, dtype, bytes, sizes);
+  } else {
+    k = at::empty(sizes, options.dtype(dtype));
+    v = at::empty(sizes, options.dtype(dtype));
+  }
   if (p.tokens > 0) {
     fill(p, c);
     p.k = k.data_ptr();
@@ -441,13 +462,7 @@ PyObject* kv4_extend(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const auto options = at::TensorOptions().device(device).dtype(at::kByte);
   const at::Tensor room = p.batch > 0 ? at::empty({from[4]}, options) : at::zeros({from[4]}, options);
   at::Tensor out[4];
-  for (int i = 0; i < 4; ++i) {
-    const auto dtype = c10::scalarTypeToTypeMeta(i < 2 ? at::kLong : at::kInt);
-    out[i] = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(room.storage()), room.key_set(), dtype);
-    c10::TensorImpl* const impl = out[i].unsafeGetTensorImpl();
-    impl->set_storage_offset(from[i] / (i < 2 ? 8 : 4));
-    impl->set_sizes_contiguous(c10::IntArrayRef(length[i]));
-  }
+  for (int i = 0; i < 4; ++i) out[i] = part_of(room, i < 2 ? at::kLong : at::kInt, from[i], length[i]);
   p.lens = static_cast<const int32_t*>(lens.const_data_ptr());
   p.slots = static_cast<int64_t*>(out[0].data_ptr());
   p.positions = static_cast<int64_t*>(out[1].data_ptr());
